@@ -371,6 +371,129 @@ int yahkv_slot_check(const yahkv_geometry* g, const void* header, size_t slot_by
 int yahkv_slot_unpack(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* table_row, int32_t n_pages,
                       const void* slot, void* stream);
 
+/* ---- rotary positions in general, alone and fused with the append --------------------------------------------------------
+ * yahkv_append_rope above has one layout, one frequency rule, angles in f32 and a token's cache slot for its position. These
+ * functions take either layout, a part of the head anywhere in it, scaled frequencies, and positions of their own: after an
+ * eviction a token's slot no longer says where it stood. (The reference has the one form only,
+ * engine/gpu/loom/yah_fused_qk_rope_f32.loom:1-10.)
+ * Pair p of a row is turned by the angle a = pos * f_p, with c = magnitude * cos a and s = magnitude * sin a:
+ *   x' = x c - y s, y' = y c + x s
+ * where (x, y) are dims (first_dim + p, first_dim + rotary_dim / 2 + p) in the HALF layout and (first_dim + 2 p,
+ * first_dim + 2 p + 1) in the INTERLEAVED one; the other dims pass through. With `normalise` every row first becomes
+ * (x * rsqrt(sum x^2 / head_dim + eps)) * weight, all its dims.
+ * Frequencies are held in turns as binary fractions, f_p / (2 pi) * 2^64: an integer product with the position, modulo
+ * 2^64, is the angle's fraction of a turn without any loss however far the position, so angles are exact to f32's last
+ * bits at every int32 position, also negative ones. */
+typedef enum yahkv_rotary_layout { YAHKV_ROTARY_HALF = 0, YAHKV_ROTARY_INTERLEAVED = 1 } yahkv_rotary_layout;
+typedef enum yahkv_rotary_scaling {
+  YAHKV_ROTARY_PLAIN = 0,   /* f_p = theta^(-2 p / rotary_dim) */
+  YAHKV_ROTARY_LINEAR = 1,  /* f_p / factor: positions interpolated */
+  YAHKV_ROTARY_NTK = 2,     /* theta * factor^(rotary_dim / (rotary_dim - 2)) in place of theta */
+  YAHKV_ROTARY_YARN = 3,    /* f_p / factor below `low` turns within original_len, f_p above `high`, a ramp over the pairs
+                               between; magnitude 0.1 ln(factor) + 1 */
+  YAHKV_ROTARY_BANDS = 4    /* the same three bands with the blend linear in the turns, magnitude 1 */
+} yahkv_rotary_scaling;
+typedef struct yahkv_rotary_spec {
+  int32_t rotary_dim;   /* a multiple of 8, at least 8 */
+  int32_t scaling;      /* yahkv_rotary_scaling */
+  double theta;         /* > 1 */
+  double factor;        /* at least 1; ignored by PLAIN */
+  double original_len;  /* YARN, BANDS: the context the frequencies were trained on, > 0 */
+  double low, high;     /* YARN, BANDS: turns within original_len, 0 < low < high (for example 1 and 32, 1 and 4) */
+} yahkv_rotary_spec;
+/* Host: the frequency table, turns[rotary_dim / 2], and the scaling's magnitude. Copy the table to the device once. */
+int yahkv_rotary_table(const yahkv_rotary_spec* spec, uint64_t* turns, float* magnitude);
+typedef struct yahkv_rotary {
+  const uint64_t* turns;  /* device [rotary_dim / 2], 8-byte aligned */
+  int32_t rotary_dim;     /* a multiple of 8, 8 .. head_dim - first_dim */
+  int32_t first_dim;      /* a multiple of 4 */
+  int32_t layout;         /* yahkv_rotary_layout */
+  float magnitude;
+  int32_t normalise;      /* not 0: head RMSNorm first */
+  float eps;
+  const float* q_weight;  /* device f32 [head_dim], 16-byte aligned, or NULL (ones) */
+  const float* k_weight;
+} yahkv_rotary;
+/* Rows of head_dim values, [n_seqs][n_new][n_heads] of them at element strides of their own (slices of a fused projection,
+ * head-major tensors). data is 16-byte aligned and every stride a multiple of 16 bytes. */
+typedef struct yahkv_rows {
+  void* data;
+  int32_t dtype;    /* yahkv_dtype */
+  int32_t n_heads;
+  int64_t seq_stride, token_stride, head_stride;
+} yahkv_rows;
+/* Rotates q rows and / or k rows (either pair may be NULL) into rows of any dtype; token t of sequence s stands at
+ * positions[s][t] (device int32 [n_seqs][n_new]). Source and destination may be the same rows (same address, strides and
+ * dtype), else they must not overlap. head_dim: a multiple of 8 up to 512. For pools without a fused append (yahkv_f16_*,
+ * yahkv_kv8_*): rotate, then append. */
+int yahkv_rotary_apply(const yahkv_rotary* rotary, int32_t head_dim, const int32_t* positions, int32_t n_seqs, int32_t n_new,
+                       const yahkv_rows* q_src, const yahkv_rows* q_dst, const yahkv_rows* k_src, const yahkv_rows* k_dst,
+                       void* stream);
+/* yahkv_append with the rotation of K (and of q, if given) fused in: token t of sequence s goes to cache slot start_pos[s]
+ * + t and is turned by positions[s][t] (NULL: by its slot). k and v have n_kv_heads rows a token, q_src and q_dst (both or
+ * neither) n_q_heads; k, v and q_src are of one dtype. k_out: [n_seqs][n_new][n_kv_heads][D] f32 or NULL, the rotated K
+ * rows. Rows at or past n_valid[s] are neither written nor rotated. */
+int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
+                        int32_t page_table_stride, const int32_t* start_pos, const int32_t* n_valid, int32_t n_seqs,
+                        int32_t n_new, const yahkv_rotary* rotary, const int32_t* positions, const yahkv_rows* k,
+                        const yahkv_rows* v, const yahkv_rows* q_src, const yahkv_rows* q_dst, float* k_out, void* stream);
+
+/* ---- attention over a shared prefix ---------------------------------------------------------------------------------------
+ * Decode attention for a batch whose sequences begin with prefixes they share, each prefix's keys read and decoded once for
+ * all the query rows that see them. Sequences group_first[j] .. group_first[j + 1] - 1 form group j (device int32
+ * [n_groups + 1], rising from 0 to n_seqs), and their page-table rows name the same pages for the prefix's first
+ * 64 * floor(shared_len[j] / 64) tokens (device int32 [n_groups]; forks share a prefix's full pages): these are read
+ * through the row of the group's first sequence, the rest of every sequence through its own row. A sequence
+ * shorter than those tiles is read through its own row alone (max_tail_len has to cover it); one of length 0 gives zeros. Results are those of yahkv_decode_attend up to the order of the sums
+ * (both within 2e-3 of exact arithmetic on the dequantized K / V; a 16-bit out adds its own rounding).
+ *   q, gate    as yahkv_decode_attend
+ *   out        [n_seqs][n_q_heads][D] of out_dtype (F32, F16 or BF16), 16-byte aligned
+ *   max_shared_len, max_tail_len  host bounds: of shared_len[] (a longer prefix is cut to the bound and the rest counts as
+ *              tail) and of the tokens any sequence reads through its own row (more are cut off, as lengths above
+ *              max_seq_len are elsewhere)
+ * softmax_scale > 0. Three dispatches: prefixes, tails (yahkv_decode_part), the merge. */
+size_t yahkv_decode_shared_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t n_groups, int32_t max_shared_len,
+                                           int32_t max_tail_len);
+int yahkv_decode_attend_shared(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
+                               int32_t page_table_stride, const int32_t* seq_len, int32_t n_seqs,
+                               const int32_t* group_first, const int32_t* shared_len, int32_t n_groups,
+                               int32_t max_shared_len, int32_t max_tail_len, const void* q, int32_t q_dtype,
+                               float softmax_scale, const float* gate, void* out, int32_t out_dtype, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* ---- eviction by accumulated attention weight ----------------------------------------------------------------------------
+ * Decode attention that also leaves what each key weighed: for t < seq_len[s]
+ *   weights_out[s][h][t] = decay * weights_in[s][h][t] + sum over kv head h's query heads of softmax weight t
+ * with f32 rows [n_seqs][n_kv_heads][weights_stride]; weights_in may be NULL (zeros) or weights_out itself; entries at or
+ * past the length are not touched. out is of out_dtype (F32, F16 or BF16); other arguments as yahkv_decode_attend. The weights
+ * are f32 throughout (scores from the exact codes), whatever out_dtype; lengths above max_seq_len or above weights_stride
+ * are clamped, and max_seq_len may not exceed weights_stride. Three dispatches. */
+size_t yahkv_decode_weights_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t max_seq_len);
+int yahkv_decode_attend_weights(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
+                                int32_t page_table_stride, const int32_t* seq_len, int32_t n_seqs, int32_t max_seq_len,
+                                const void* q, int32_t q_dtype, float softmax_scale, const float* gate, void* out,
+                                int32_t out_dtype, const float* weights_in, float* weights_out, int32_t weights_stride,
+                                float decay, void* workspace, size_t workspace_bytes, void* stream);
+/* The keys each kv head keeps when its sequence is cut to `budget` tokens: the first `sink`, the last `recent`, and of the
+ * others those of largest weight (ties: the lowest position first; negative and NaN weights count as zero), written in
+ * rising order to kept[s][h][0 .. n_kept[s]), -1 from there to budget; n_kept[s] = min(length, budget). A sequence of at most
+ * `budget` tokens keeps all. 0 <= sink + recent <= budget. weights as above; lengths are clamped to max_seq_len. kept:
+ * device int32 [n_seqs][n_kv_heads][budget]; n_kept: device int32 [n_seqs]. */
+int yahkv_evict_select(const yahkv_geometry* g, const int32_t* seq_len, int32_t n_seqs, int32_t max_seq_len,
+                       const float* weights, int32_t weights_stride, int32_t budget, int32_t sink, int32_t recent,
+                       int32_t* kept, int32_t* n_kept, void* stream);
+/* Moves the kept tokens together: codes and scales of token kept[s][h][i] of kv head h go, bit for bit, to slot i of
+ * sequence s's new pages dst_table[s][0 .. ceil(budget / PT)), and weights_in[s][h][kept[s][h][i]] to weights_out[s][h][i]
+ * (both NULL: no weights). Slots at or past n_kept[s] are left as they are. New pages must not be pages that any source
+ * row of this call names: sources may be shared with other sequences, so nothing is moved in place; take fresh pages from the
+ * allocator, upload their row in place of the old one, and free the old pages behind the call in stream order. Afterwards the sequence
+ * is n_kept[s] tokens long, and its next token goes to slot n_kept[s] at its own position (yahkv_rotary_append). Kept
+ * positions are clamped to the table, pages to the pool. */
+int yahkv_evict_compact(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
+                        int32_t page_table_stride, const int32_t* kept, const int32_t* n_kept, int32_t n_seqs,
+                        int32_t budget, const int32_t* dst_table, int32_t dst_table_stride, const float* weights_in,
+                        int32_t weights_in_stride, float* weights_out, int32_t weights_out_stride, void* stream);
+
 /* ---- unquantized f16 pools: the reference's fp16 twins of the decode path ------------------------------------------
  * yah_dattn_kvappend (engine/gpu/loom/tools/gen_decode_attn.py:30-94), yah_dattn_part (:97-335) and yah_dattn_reduce
  * (:338-411) on pools of f16 K and f16 V^T, with the page table, positions, clamping and argument meaning of the

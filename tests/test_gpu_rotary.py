@@ -1,0 +1,224 @@
+"""Rotary positions on the GPU (yahkv_rotary_apply, yahkv_rotary_append) against the definition in float64.
+
+Tolerance of an f32 result, in u = 2^-24 of the larger of the row's magnitudes: the sum of up to 512 squares 8 + 6 steps,
+division, root and reciprocal 3, two products 2: 19, halved for the sum by the root, so 12 u on a normalised value; cosine and
+sine 4 u (two units of the last place at most), the remainder's rounding pi / 4 u, the magnitude u; a product and a sum 2 u: 20 u
+on each of two terms, 40 u = 2.4e-6 of (|x| + |y|) at most, taken as 2.4e-6 of twice the row's largest value times the
+magnitude. A 16-bit result adds half a step of its own value, finfo.eps / 2."""
+import math
+
+import numpy as np
+import pytest
+
+import oracle
+from helpers import make_tables
+from test_host_serving import frequencies
+
+pytestmark = pytest.mark.gpu
+SPEC = dict(none=0, linear=1, ntk=2, yarn=3, bands=4)
+
+
+def want_rows(x, pos, dim, layout, scaling, first=0, weight=None, eps=1e-6, normalise=False, theta=1e4):
+    """x float64 [n][t][heads][D], pos [n][t]."""
+    low, high = (1.0, 4.0) if scaling == "bands" else (1.0, 32.0)
+    f = frequencies(dim, SPEC[scaling], theta, 8.0, 4096.0, low, high)
+    mag = 0.1 * math.log(8.0) + 1 if scaling == "yarn" else 1.0
+    # angles of far positions in extended precision
+    a = (np.asarray(pos, np.longdouble)[..., None, None] * f.astype(np.longdouble)) % np.longdouble("6.28318530717958647692528676655900577")
+    c, s = np.cos(a).astype(np.float64) * mag, np.sin(a).astype(np.float64) * mag
+    x = np.array(x, np.float64)
+    if normalise:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
+        if weight is not None:
+            x = x * weight
+    out = x.copy()
+    i0 = first + (np.arange(dim // 2) if layout == "half" else 2 * np.arange(dim // 2))
+    i1 = i0 + (dim // 2 if layout == "half" else 1)
+    out[..., i0] = x[..., i0] * c - x[..., i1] * s
+    out[..., i1] = x[..., i1] * c + x[..., i0] * s
+    return out
+
+
+def close(torch, got, want, dtype):
+    got = got.double().cpu().numpy()
+    half = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    tiny = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}[dtype]        # half a subnormal step
+    tol = 2.4e-6 * 2 * 1.3 * np.abs(want).max(-1, keepdims=True) + half * np.abs(want) * 1.001 + tiny
+    assert got.shape == want.shape and np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+def make(yahkv, dim, layout, scaling, **kw):
+    low, high = (1.0, 4.0) if scaling == "bands" else (1.0, 32.0)
+    return yahkv.Rotary(dim, kw.pop("theta", 1e4), layout=layout, scaling=scaling, factor=8.0, original_len=4096.0, low=low, high=high, **kw)
+
+
+@pytest.mark.parametrize("scaling", sorted(SPEC))
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_scalings_and_far_positions(yahkv, torch_gpu, layout, scaling):
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    pos = np.array([[0], [1], [-1], [4095], [123456], [2 ** 31 - 1], [-2 ** 31], [1000003]])
+    q = torch.randn(8, 1, 3, 128, generator=gen, device="cuda")
+    k = torch.randn(8, 1, 1, 128, generator=gen, device="cuda")
+    r = make(yahkv, 128, layout, scaling)
+    qo, ko = yahkv.rotary_rows(r, torch.tensor(pos, dtype=torch.int32, device="cuda"), q, k)
+    # the frequencies are doubles on both sides, rounded apart: up to 2^-46 relative (tested on the host), which at position
+    # 2^31 is 3e-5 radians; nearer positions show it less
+    spread = np.abs(pos)[..., None, None] * 64 * 2.0 ** -53
+    for got, x in ((qo, q), (ko, k)):
+        want = want_rows(x.cpu().numpy(), pos, 128, layout, scaling)
+        tol = (2.4e-6 * 2.6 + 2.6 * spread) * np.abs(want).max(-1, keepdims=True)
+        assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.parametrize("d,dim,first", [(8, 8, 0), (40, 16, 8), (64, 32, 32), (80, 80, 0), (96, 64, 4), (128, 128, 0), (192, 64, 128),
+                                         (256, 64, 0), (256, 256, 0), (512, 512, 0), (512, 128, 100)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_part_of_the_head_and_types(yahkv, torch_gpu, layout, d, dim, first):
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda").manual_seed(d + dim)
+    pos = torch.randint(0, 5000, (2, 3), generator=gen, device="cuda", dtype=torch.int32)
+    w = 1 + 0.3 * torch.randn(d, generator=gen, device="cuda")
+    for n, (src, dst) in enumerate(((torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float16))):
+        q = torch.randn(2, 3, 5, d, generator=gen, device="cuda").to(src)
+        k = torch.randn(2, 3, 2, d, generator=gen, device="cuda").to(src)
+        r = make(yahkv, dim, layout, "none", first_dim=first, normalise=n != 1, q_weight=w if n == 0 else None, k_weight=w)
+        qo, ko = yahkv.rotary_rows(r, pos, q, k, out_dtype=dst)
+        p = pos.cpu().numpy()
+        w64 = w.double().cpu().numpy()
+        close(torch, qo, want_rows(q.double().cpu().numpy(), p, dim, layout, "none", first, w64 if n == 0 else None, normalise=n != 1), dst)
+        close(torch, ko, want_rows(k.double().cpu().numpy(), p, dim, layout, "none", first, w64, normalise=n != 1), dst)
+
+
+@pytest.mark.parametrize("n,new", [(1, 1), (3, 1), (1, 1100), (2, 5)])
+def test_strided_in_place_and_alone(yahkv, torch_gpu, n, new):
+    """Slices of one fused projection, a head-major tensor, rotation in place, k without q; the rest of the buffer untouched."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(n, new, 12, 128, generator=gen, device="cuda").to(torch.bfloat16)
+    before = x.clone()
+    pos = torch.randint(0, 300000, (n, new), generator=gen, device="cuda", dtype=torch.int32)
+    r = make(yahkv, 64, "half", "linear", normalise=True)
+    q, k = x[:, :, :8], x[:, :, 8:10]
+    want_q = want_rows(before[:, :, :8].double().cpu().numpy(), pos.cpu().numpy(), 64, "half", "linear", normalise=True)
+    want_k = want_rows(before[:, :, 8:10].double().cpu().numpy(), pos.cpu().numpy(), 64, "half", "linear", normalise=True)
+    qo, ko = yahkv.rotary_rows(r, pos, q, k)                                  # out of place: strided in, dense out
+    close(torch, qo, want_q, torch.bfloat16)
+    close(torch, ko, want_k, torch.bfloat16)
+    head_major = torch.zeros(n, 8, new, 128, device="cuda", dtype=torch.bfloat16).transpose(1, 2)
+    yahkv.rotary_rows(r, pos, q, q_out=head_major)
+    assert torch.equal(head_major, qo)
+    only = yahkv.rotary_rows(r, pos, k=k)
+    assert only[0] is None and torch.equal(only[1], ko)
+    assert torch.equal(x, before)
+    yahkv.rotary_rows(r, pos, q, k, q_out=q, k_out=k)                         # in place
+    assert torch.equal(x[:, :, :8], qo) and torch.equal(x[:, :, 8:10], ko) and torch.equal(x[:, :, 10:], before[:, :, 10:])
+
+
+def test_untouched_dims_pass_through_infinities(yahkv, torch_gpu):
+    """Dims that are not rotated are the source's bits, NaN and infinities among them; a pair with one is not finite."""
+    torch = torch_gpu
+    x = torch.randn(1, 1, 2, 64, device="cuda")
+    x[0, 0, 0, 40], x[0, 0, 1, 63], x[0, 0, 1, 0] = float("inf"), float("nan"), float("inf")
+    y, _ = yahkv.rotary_rows(make(yahkv, 32, "half", "none"), torch.tensor([[5]], dtype=torch.int32, device="cuda"), x)
+    assert torch.equal(y[..., 32:].view(torch.int32), x[..., 32:].view(torch.int32))
+    assert torch.isfinite(y[0, 0, 0, :32]).all() and not torch.isfinite(y[0, 0, 1, [0, 16]]).any()
+
+
+def append_case(yahkv, torch, fmt, n_q, n_kv, hd, pt, starts, new, layout, dim, first, src, seed, n_valid=None, far=0):
+    rng = np.random.default_rng(seed)
+    pages = [(s + new + pt - 1) // pt for s in starts]
+    g = oracle.geometry(fmt, n_q, n_kv, hd, pt, sum(pages) + 1)
+    table = make_tables(rng, pages, g.n_pages)
+    n = len(starts)
+    x = torch.from_numpy(rng.standard_normal((n, new, n_q + 2 * n_kv, hd)).astype(np.float32)).cuda().to(src)
+    dev = yahkv.DevicePools(yahkv.geometry(fmt, n_q, n_kv, hd, pt, g.n_pages), fill=0x5A)
+    t = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+    pos = np.asarray(starts)[:, None] + np.arange(new) + far
+    r = make(yahkv, dim, layout, "yarn", first_dim=first, normalise=True)
+    k_out = torch.full((n, new, n_kv, hd), float("nan"), device="cuda")
+    q_out = yahkv.rotary_append(dev, t(table), t(starts), r, x[:, :, n_q:n_q + n_kv], x[:, :, n_q + n_kv:], x[:, :, :n_q],
+                                positions=t(pos) if far else None, k_out=k_out, n_valid=None if n_valid is None else t(n_valid))
+    torch.cuda.synchronize()
+    return g, table, x, dev, pos, k_out, q_out
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("fmt,n_q,n_kv,hd,pt,starts,new,dim,first,far", [
+    (8, 24, 4, 256, 64, [0, 37, 63], 1, 256, 0, 900000), (4, 8, 2, 128, 16, [15, 16, 0], 1, 64, 64, 12345),
+    (8, 8, 8, 128, 32, [0, 5, 100], 7, 128, 0, 0), (8, 8, 1, 256, 16, [3, 0, 40], 21, 64, 4, 70000),
+    (4, 32, 8, 128, 64, [0, 1, 64], 130, 32, 0, 500), (8, 24, 4, 256, 64, [10, 0, 64], 530, 64, 0, 100000)])
+def test_append(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, starts, new, dim, first, far, layout):
+    """The rows against the definition; the pools bit for bit the oracle's quantization of the kernel's own rotated rows; rows
+    of a padded chunk and everything else in the pools as they were."""
+    torch = torch_gpu
+    nv = [new, max(new // 2, 1), new] if new > 1 else None
+    src = torch.bfloat16 if fmt == 8 else torch.float16
+    g, table, x, dev, pos, k_out, q_out = append_case(yahkv, torch, fmt, n_q, n_kv, hd, pt, starts, new, layout, dim, first, src,
+                                                       new + hd, nv, far)
+    x64 = x.double().cpu().numpy()
+    want_q = want_rows(x64[:, :, :n_q], pos, dim, layout, "yarn", first, normalise=True)
+    want_k = want_rows(x64[:, :, n_q:n_q + n_kv], pos, dim, layout, "yarn", first, normalise=True)
+    valid = nv or [new] * 3
+    for s in range(3):
+        close(torch, q_out[s, :valid[s]], want_q[s, :valid[s]], torch.float32)
+        close(torch, k_out[s, :valid[s]], want_k[s, :valid[s]], torch.float32)
+        assert torch.isnan(k_out[s, valid[s]:]).all()
+    host = oracle.HostPools(g, fill=0x5A)
+    oracle.append(host, table, starts, valid, np.nan_to_num(k_out.cpu().numpy()), np.ascontiguousarray(x64[:, :, n_q + n_kv:], np.float32))
+    got = dev.numpy()
+    for name, want in host.arrays().items():
+        assert np.array_equal(got[name], want), name
+
+
+def test_append_without_queries_or_norm_equals_rotate_then_append(yahkv, torch_gpu):
+    torch = torch_gpu
+    rng = np.random.default_rng(4)
+    g = yahkv.geometry(8, 8, 2, 128, 16, 8)
+    table = torch.from_numpy(rng.permutation(8).astype(np.int32).reshape(2, 4)).cuda()
+    start = torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([[70000, 5], [9, 2 ** 30]], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(2, 2, 2, 128, device="cuda") for _ in range(2))
+    r = make(yahkv, 96, "interleaved", "bands", first_dim=32)
+    a, b = yahkv.DevicePools(g), yahkv.DevicePools(g)
+    k_out = torch.empty_like(k)
+    assert yahkv.rotary_append(a, table, start, r, k, v, positions=pos, k_out=k_out) is None
+    _, rows = yahkv.rotary_rows(r, pos, k=k)
+    # the two kernels may contract a product and a sum differently: one rounding apart
+    assert (rows - k_out).abs().max() <= 4 * 2.0 ** -24 * k.abs().max()
+    yahkv.append(b, table, start, k_out, v)
+    for name in ("kq", "ks", "vq", "vs"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+
+
+def test_replays_from_a_graph_on_another_stream(yahkv, torch_gpu):
+    torch = torch_gpu
+    g = yahkv.geometry(8, 24, 4, 256, 64, 4)
+    table = torch.arange(4, dtype=torch.int32, device="cuda").reshape(4, 1)
+    start = torch.tensor([0, 5, 63, 7], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([[1], [2], [3], [99999]], dtype=torch.int32, device="cuda")
+    x = torch.randn(4, 1, 32, 256, device="cuda").to(torch.bfloat16)
+    r = make(yahkv, 64, "half", "yarn", normalise=True)
+    dev = yahkv.DevicePools(g)
+    q_out = torch.empty(4, 1, 24, 256, device="cuda", dtype=torch.bfloat16)
+    step = lambda: yahkv.rotary_append(dev, table, start, r, x[:, :, 24:28], x[:, :, 28:], x[:, :, :24], positions=pos, q_out=q_out)
+    step()
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for i in range(3):
+        x.copy_(torch.randn(4, 1, 32, 256, device="cuda"))
+        pos.add_(1)
+        step()
+        want = [t.clone() for t in (q_out, dev.kq, dev.ks, dev.vq, dev.vs)]
+        for t in (q_out, dev.kq, dev.ks, dev.vq, dev.vs):
+            t.zero_() if t is not q_out else t.fill_(float("nan"))
+        graph.replay()
+        first = [t.clone() for t in (q_out, dev.kq, dev.ks, dev.vq, dev.vs)]
+        assert torch.equal(first[0], want[0]), i
+        dev.kq.zero_(), dev.ks.zero_(), dev.vq.zero_(), dev.vs.zero_()
+        step()
+        for name, t in zip(("kq", "ks", "vq", "vs"), first[1:]):
+            assert torch.equal(getattr(dev, name), t), name

@@ -1,0 +1,185 @@
+"""Decode attention over shared prefixes (yahkv_decode_attend_shared) against the closed form in float64, and against the
+plain decode attention on the same tables.
+
+Tolerance: the library's 2e-3 of the largest value (K, V and the softmax numerators enter the matrix unit as f16, half a step
+2^-11 each, over sums of independent terms); a 16-bit output adds half a step of its own value, finfo.eps / 2."""
+import numpy as np
+import pytest
+
+import oracle
+from helpers import to_bf16_f32
+from test_gpu_decode import closed
+
+pytestmark = pytest.mark.gpu
+TOL = 2e-3
+
+
+def batch(yahkv, torch, fmt, n_q, n_kv, hd, pt, groups, seed, fill=0x7F, spare=2):
+    """groups: [(shared_len, [lengths])]. Full pages of a prefix are shared, the rest is every sequence's own."""
+    rng = np.random.default_rng(seed)
+    lens = [n for _, ls in groups for n in ls]
+    pages_of = lambda n: (n + pt - 1) // pt
+    total = sum(sh // pt + sum(max(pages_of(n) - sh // pt, 0) for n in ls) for sh, ls in groups)
+    # a sequence shorter than its prefix keeps the row of the shared pages
+    g = oracle.geometry(fmt, n_q, n_kv, hd, pt, total + spare)
+    perm, at = rng.permutation(g.n_pages).astype(np.int32), 0
+    table = np.zeros((len(lens), max(max(pages_of(max(n, sh)) for sh, ls in groups for n in ls), 1)), np.int32)
+    host = oracle.HostPools(g, fill=fill)
+    s = 0
+    rows = lambda n: to_bf16_f32(rng.standard_normal((1, n, n_kv, hd)))
+    for sh, ls in groups:
+        common, at = perm[at:at + sh // pt], at + sh // pt
+        pk, pv = rows(sh) if sh else None, rows(sh) if sh else None
+        for n in ls:
+            table[s, :len(common)] = common
+            own = max(pages_of(n) - len(common), 0)
+            table[s, len(common):len(common) + own] = perm[at:at + own]
+            at += own
+            if n:
+                k, v = rows(n), rows(n)
+                m = min(sh, n)
+                if m:
+                    k[:, :m], v[:, :m] = pk[:, :m], pv[:, :m]
+                oracle.append(host, table[s:s + 1], [0], None, k, v)
+            s += 1
+        if sh // pt:  # the prefix's pages are whole even where no sequence reaches their end
+            oracle.append(host, table[s - 1:s], [0], None, pk[:, :sh // pt * pt], pv[:, :sh // pt * pt])
+    dev = yahkv.DevicePools(yahkv.geometry(fmt, n_q, n_kv, hd, pt, g.n_pages))
+    dev.load(host.arrays())
+    first = np.cumsum([0] + [len(ls) for _, ls in groups])
+    t = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+    shared = [sh for sh, _ in groups]
+    tail = max([1] + [n - (sh // 64 * 64 if n >= sh // 64 * 64 else 0) for sh, ls in groups for n in ls])
+    q = torch.from_numpy(rng.standard_normal((len(lens), n_q, hd)).astype(np.float32)).cuda()
+    return g, table, host, dev, lens, q, dict(table=t(table), seq_len=t(lens), group_first=t(first), shared_len=t(shared),
+                                              max_shared_len=max(shared), max_tail_len=tail)
+
+
+def check(torch, got, want, dtype):
+    got = got.double().cpu().numpy()
+    half = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
+    assert np.all(np.isfinite(got))
+    err = np.abs(got - want)
+    assert np.all(err <= TOL * np.abs(want).max() + half * 1.002 * np.abs(want)), float(err.max() / np.abs(want).max())
+
+
+HEADS = [(24, 4, 256), (32, 8, 128), (8, 8, 128), (8, 1, 256), (3, 1, 128)]
+
+
+@pytest.mark.parametrize("fmt,pt", [(8, 64), (8, 16), (4, 32), (4, 64)])
+@pytest.mark.parametrize("n_q,n_kv,hd", HEADS)
+def test_one_prefix(yahkv, torch_gpu, n_q, n_kv, hd, fmt, pt):
+    torch = torch_gpu
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, fmt, n_q, n_kv, hd, pt, [(300, [300, 301, 420, 364, 999])], fmt * pt + hd)
+    scale = hd ** -0.5
+    for kind, dtype in ((torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)):
+        x = q.to(kind)
+        want = closed(g, table, host, lens, x.double().cpu().numpy(), scale)
+        check(torch, yahkv.decode_attend_shared(dev, q=x, scale=scale, out_dtype=dtype, **a), want, dtype)
+
+
+@pytest.mark.parametrize("groups", [
+    [(0, [1])], [(0, [0, 5, 64, 65])], [(63, [63, 64, 200])], [(64, [64, 64, 65])], [(65, [65, 65])], [(128, [128])],
+    [(129, [0, 1, 63, 64, 127, 128, 129, 400])],                                     # some shorter than the prefix, one empty
+    [(1000, [0, 0, 0])],                                                             # nothing but empty ones
+    [(200, [200, 264]), (0, [77]), (640, [700] * 9), (64, [10, 64, 3])],             # groups side by side, one without a prefix
+    [(192, [250 + i for i in range(23)])], [(3000, [3000 + i for i in range(45)])],  # more rows than a workgroup's
+    [(64 * i + 64, [64 * i + 70]) for i in range(9)]])                               # every sequence a group of its own
+def test_lengths_and_groups(yahkv, torch_gpu, groups):
+    torch = torch_gpu
+    n_q, n_kv, hd, pt = 12, 2, 128, 32
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, n_q, n_kv, hd, pt, groups, len(groups) + groups[0][0])
+    gate = torch.randn(len(lens), n_q, hd, device="cuda")
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), 0.1, gate.double().cpu().numpy())
+    got = yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, gate=gate, **a)
+    check(torch, got, want, torch.float32)
+    for s, n in enumerate(lens):
+        assert n > 0 or not got[s].any()
+    if max(lens) == 0:
+        return
+    plain = yahkv.decode_attend(dev, a["table"], a["seq_len"], max(lens), q.half(), 0.1, gate=gate)
+    check(torch, got, plain.double().cpu().numpy(), torch.float32)
+    # larger host bounds than needed change nothing but the sums' order
+    a.update(max_shared_len=a["max_shared_len"] + 5000, max_tail_len=a["max_tail_len"] + 777)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, gate=gate, **a), want, torch.float32)
+
+
+def test_bounds_clamp(yahkv, torch_gpu):
+    """A prefix beyond max_shared_len counts as tail; a shared_len that is negative or past the table is cut to it."""
+    torch = torch_gpu
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 8, 2, 128, 16, [(256, [256, 300, 280])], 5)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), 0.1)
+    b = dict(a, max_shared_len=128, max_tail_len=300 - 128)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **b), want, torch.float32)
+    b = dict(a, shared_len=torch.tensor([-7], dtype=torch.int32, device="cuda"), max_tail_len=300)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **b), want, torch.float32)
+    # the table reaches 19 pages of 16 tokens: 304, of which whole tiles 256
+    b = dict(a, shared_len=torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda"), max_shared_len=2 ** 31 - 1 - 64)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **b), want, torch.float32)
+
+
+def test_large_values_stay_finite(yahkv, torch_gpu):
+    """Blocks of values up to the largest f16 scale times 127: the products saturate instead of becoming infinite."""
+    torch = torch_gpu
+    g = yahkv.geometry(8, 8, 1, 128, 64, 3)
+    dev = yahkv.DevicePools(g, fill=1)
+    dev.vs.view(torch.float16).fill_(60000.0)
+    dev.ks.view(torch.float16).fill_(2.0)
+    dev.vq.view(torch.int8).fill_(127)
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 8, 128, device="cuda").half()
+    out = yahkv.decode_attend_shared(dev, torch.tensor([[0, 1], [0, 2]], dtype=torch.int32, device="cuda"), t(64, 64), t(0, 2), t(64),
+                                     64, 64, q, 0.1)
+    assert torch.all((out - 65504.0).abs() <= 65504.0 * TOL)
+
+
+def test_non_finite_keys_stay_with_those_who_see_them(yahkv, torch_gpu):
+    """A NaN scale behind every sequence's end, or in prefix keys that only the longer sequences have, leaves the others alone."""
+    torch = torch_gpu
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 8, 2, 128, 64, [(192, [192, 100, 300, 0])], 6)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), 0.1)
+    nan = torch.tensor(float("nan"), device="cuda", dtype=torch.float16)
+    vs, ks = dev.vs.view(torch.float16).view(-1, 2, 4, 64), dev.ks.view(torch.float16).view(-1, 2, 64, 4)
+    vs[table[2, 4], :, :, 300 - 256:], ks[table[2, 4], :, 300 - 256:] = nan, nan      # behind the longest sequence's end
+    got = yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **a)
+    check(torch, got, want, torch.float32)
+    vs[table[0, 2], 0, 1, 5] = nan                                                    # key 133: not sequence 1's
+    got = yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **a)
+    assert torch.isnan(got[[0, 2]][:, :4, 32:64]).all() and torch.isfinite(got[1]).all() and not got[3].any()
+    check(torch, got[1], want[1], torch.float32)
+
+
+def test_same_bits_twice_and_from_a_graph(yahkv, torch_gpu):
+    torch = torch_gpu
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 24, 4, 256, 64, [(640, [700 + 9 * i for i in range(7)]), (64, [500, 64])], 8)
+    x = q.to(torch.bfloat16)
+    ws = torch.empty(yahkv.decode_shared_workspace_bytes(dev.geom, 9, 2, a["max_shared_len"], a["max_tail_len"]), dtype=torch.uint8, device="cuda")
+    out = torch.empty(x.shape, device="cuda")
+    step = lambda: yahkv.decode_attend_shared(dev, q=x, scale=0.0625, out=out, workspace=ws, **a)
+    step()
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for i in range(3):
+        x.copy_(torch.randn(x.shape, device="cuda"))
+        a["seq_len"].add_(i)                  # lengths live on the device (the new keys were never written: NaN, so bits are compared)
+        ws.random_(0, 256)
+        step()
+        want = out.clone()
+        out.fill_(float("nan"))
+        ws.random_(0, 256)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int32), want.view(torch.int32)) and (i or torch.isfinite(out).all()), i
+        a["seq_len"].sub_(i)
+
+
+def test_workspace_too_small_is_refused(yahkv, torch_gpu):
+    torch = torch_gpu
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 8, 2, 128, 16, [(64, [70])], 9)
+    with pytest.raises(yahkv.YahkvError) as e:
+        yahkv.decode_attend_shared(dev, q=q, scale=0.1, workspace=torch.empty(64, dtype=torch.uint8, device="cuda"), **a)
+    assert e.value.status == -4

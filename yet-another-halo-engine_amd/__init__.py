@@ -51,6 +51,22 @@ class Rope(C.Structure):
                 ("q_weight", C.c_void_p)]
 
 
+class RotarySpec(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("scaling", C.c_int32), ("theta", C.c_double), ("factor", C.c_double),
+                ("original_len", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class RotaryStruct(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("rotary_dim", C.c_int32), ("first_dim", C.c_int32), ("layout", C.c_int32),
+                ("magnitude", C.c_float), ("normalise", C.c_int32), ("eps", C.c_float), ("q_weight", C.c_void_p),
+                ("k_weight", C.c_void_p)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int32), ("n_heads", C.c_int32), ("seq_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built: run `python __graft_entry__.py build` (hipcc, gfx950)")
@@ -124,6 +140,20 @@ def _load():
                                              C.c_size_t, vp]
     lib.yahkv_kv8_decode_step.argtypes = [G, K8, i32p, i32, i32p, i32, i32, vp, vp, i32, vp, i32, C.c_float, vp, vp, vp,
                                           C.c_size_t, O, vp]
+    RT, RW = C.POINTER(RotaryStruct), C.POINTER(Rows)
+    lib.yahkv_rotary_table.argtypes = [C.POINTER(RotarySpec), vp, C.POINTER(C.c_float)]
+    lib.yahkv_rotary_apply.argtypes = [RT, i32, i32p, i32, i32, RW, RW, RW, RW, vp]
+    lib.yahkv_rotary_append.argtypes = [G, P, i32p, i32, i32p, i32p, i32, i32, RT, i32p, RW, RW, RW, RW, vp, vp]
+    lib.yahkv_decode_shared_workspace_bytes.restype = C.c_size_t
+    lib.yahkv_decode_shared_workspace_bytes.argtypes = [G, i32, i32, i32, i32]
+    lib.yahkv_decode_attend_shared.argtypes = [G, P, i32p, i32, i32p, i32, i32p, i32p, i32, i32, i32, vp, i32, C.c_float,
+                                               vp, vp, i32, vp, C.c_size_t, vp]
+    lib.yahkv_decode_weights_workspace_bytes.restype = C.c_size_t
+    lib.yahkv_decode_weights_workspace_bytes.argtypes = [G, i32, i32]
+    lib.yahkv_decode_attend_weights.argtypes = [G, P, i32p, i32, i32p, i32, i32, vp, i32, C.c_float, vp, vp, i32, vp, vp,
+                                                i32, C.c_float, vp, C.c_size_t, vp]
+    lib.yahkv_evict_select.argtypes = [G, i32p, i32, i32, vp, i32, i32, i32, i32, i32p, i32p, vp]
+    lib.yahkv_evict_compact.argtypes = [G, P, i32p, i32, i32p, i32p, i32, i32, i32p, i32, vp, i32, vp, i32, vp]
     lib.yahkv_gather_blocks.argtypes = [G, P, i32p, i32, vp, vp, vp]
     lib.yahkv_pagepool_create.restype = C.c_void_p
     lib.yahkv_pagepool_create.argtypes = [i32]
@@ -323,6 +353,17 @@ class DevicePools:
         self.ks = torch.full((b["ks"],), fill, dtype=torch.uint8, device=device)
         self.vq = torch.full((b["vq"],), fill, dtype=torch.uint8, device=device)
         self.vs = torch.full((b["vs"],), fill, dtype=torch.uint8, device=device)
+
+    @classmethod
+    def of(cls, g, kq, ks, vq, vs):
+        """Pools over buffers the caller has: contiguous tensors of any type and shape, as long as the geometry needs."""
+        import torch
+        self = cls.__new__(cls)
+        self.geom = g
+        for name, t in (("kq", kq), ("ks", ks), ("vq", vq), ("vs", vs)):
+            _need(t.is_contiguous(), f"pools: {name} is not contiguous")
+            setattr(self, name, t.view(-1).view(torch.uint8))
+        return self
 
     def struct(self):
         return Pools(self.kq.data_ptr(), self.ks.data_ptr(), self.vq.data_ptr(), self.vs.data_ptr(),
@@ -615,6 +656,287 @@ def gather_blocks(pools, table_row, n_tokens):
     _check(lib.yahkv_gather_blocks(C.byref(g), C.byref(st), _dp(table_row), n_tokens, _dp(k), _dp(v), _stream()),
            "gather_blocks")
     return k, v
+
+
+# ---- rotary positions, shared prefixes, eviction ----------------------------------------------------------------------------
+
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+def _need(ok, what):
+    """A call the library must not see: tensors whose shape, type or device it would have to take on trust."""
+    if not ok:
+        raise YahkvError(-1, what)
+
+
+def _ints(t, shape, like, what):
+    import torch
+    _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == like and tuple(t.shape) == tuple(shape),
+          f"{what}: a contiguous int32 tensor of shape {tuple(shape)} on {like} is expected")
+
+
+def _table(t, n_seqs, like, what):
+    import torch
+    _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == like and t.dim() == 2 and t.shape[0] == n_seqs,
+          f"{what}: a contiguous int32 tensor [{n_seqs}][pages] on {like} is expected")
+
+
+def _run_on(device, call):
+    """call(stream) on torch's current stream of `device`, with that device current."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return call(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    with torch.cuda.device(device):
+        return call(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+
+
+def _out(out, shape, dtype, device, default):
+    """The caller's output tensor after a look at it, or a new one."""
+    import torch
+    if out is None:
+        return torch.empty(shape, dtype=dtype or default, device=device)
+    _need(tuple(out.shape) == tuple(shape) and out.is_contiguous() and out.device == device and
+          dtype in (None, out.dtype) and out.dtype in (torch.float32, torch.float16, torch.bfloat16),
+          f"out: a contiguous tensor of shape {tuple(shape)} on {device} is expected")
+    return out
+
+
+def _scratch(workspace, need, device):
+    import torch
+    if workspace is None:
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device,
+          "workspace: a contiguous uint8 tensor on the queries' device is expected")
+    return workspace
+
+
+def _queries(g, q, gate, pools, what):
+    import torch
+    _need(q.dtype in (torch.float32, torch.float16, torch.bfloat16) and q.is_contiguous() and q.dim() == 3 and
+          tuple(q.shape[1:]) == (g.n_q_heads, g.head_dim) and q.shape[0] > 0 and q.device == pools.kq.device,
+          f"{what}: contiguous queries [n_seqs][{g.n_q_heads}][{g.head_dim}] on the pools' device are expected")
+    _need(gate is None or (gate.dtype == torch.float32 and gate.is_contiguous() and gate.shape == q.shape and
+                           gate.device == q.device), f"{what}: gate is f32 of the queries' shape")
+
+
+class Rotary:
+    """Rotary positions: yahkv_rotary_table's frequencies on a device and how rows are turned by them. layout "half" or
+    "interleaved"; dims first_dim .. first_dim + rotary_dim - 1 of a head are rotated; scaling "none", "linear", "ntk",
+    "yarn" or "bands" (include/yahkv.h) with its factor, original context and, for the last two, the turns `low` and `high`
+    that bound its ramp; magnitude None: the scaling's own. With normalise, rows go through a head RMSNorm first (weights f32
+    [head_dim] or None)."""
+
+    def __init__(self, rotary_dim, theta, layout="half", scaling="none", factor=1.0, original_len=0.0, low=1.0, high=32.0,
+                 first_dim=0, magnitude=None, normalise=False, eps=1e-6, q_weight=None, k_weight=None, device="cuda:0"):
+        import numpy as np
+        import torch
+        _need(layout in ROTARY_LAYOUTS and scaling in ROTARY_SCALINGS, f"rotary: layout {layout!r}, scaling {scaling!r}")
+        spec = RotarySpec(rotary_dim, ROTARY_SCALINGS[scaling], theta, factor, original_len, low, high)
+        turns, own = np.zeros(max(rotary_dim // 2, 1), np.uint64), C.c_float()
+        _check(lib.yahkv_rotary_table(C.byref(spec), turns.ctypes.data, C.byref(own)), "rotary_table")
+        self.turns = torch.from_numpy(turns.view(np.int64)).to(device)
+        self.magnitude = own.value if magnitude is None else magnitude
+        for w in (q_weight, k_weight):
+            _need(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.dim() == 1 and w.device == self.turns.device),
+                  "rotary: weights are contiguous f32 rows on the table's device")
+        self.q_weight, self.k_weight = q_weight, k_weight
+        self.struct = RotaryStruct(self.turns.data_ptr(), rotary_dim, first_dim, ROTARY_LAYOUTS[layout], self.magnitude,
+                                   1 if normalise else 0, eps, None if q_weight is None else q_weight.data_ptr(),
+                                   None if k_weight is None else k_weight.data_ptr())
+
+    def check_head(self, head_dim):
+        for w in (self.q_weight, self.k_weight):
+            _need(w is None or w.numel() == head_dim, f"rotary: weights of {head_dim} values are expected")
+
+
+def _rows(t, what):
+    """A [n_seqs][n_new][heads][D] tensor, each head's values contiguous, as yahkv_rows."""
+    import torch
+    _need(t.dim() == 4 and t.dtype in (torch.float32, torch.float16, torch.bfloat16) and t.numel() > 0 and
+          (t.stride(3) == 1 or t.shape[3] == 1), f"{what}: rows [n_seqs][n_new][heads][D] with contiguous heads are expected")
+    step = [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]  # (a lone element's stride says nothing)
+    return Rows(t.data_ptr(), _dtype_code(t), t.shape[2], *step)
+
+
+def _ref(s):
+    return None if s is None else C.byref(s)
+
+
+def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_dtype=None):
+    """Rotates q and / or k, [n_seqs][n_new][heads][D] tensors at any strides of whole 16 bytes (slices of a fused projection),
+    token t of sequence s by positions[s][t] (int32). Returns (q_out, k_out), new contiguous tensors of out_dtype (the rows'
+    own by default) where none are given; q_out may be q itself. None for rows that were not given."""
+    import torch
+    first = q if q is not None else k
+    _need(first is not None and first.dim() == 4, "rotary_rows: q or k [n_seqs][n_new][heads][D]")
+    n_seqs, n_new, _, d = first.shape
+    _ints(positions, (n_seqs, n_new), first.device, "positions")
+    rotary.check_head(d)
+    _need(rotary.turns.device == first.device, "rotary_rows: the frequency table is on another device")
+    args, outs = [], []
+    for x, out in ((q, q_out), (k, k_out)):
+        if x is None:
+            _need(out is None, "rotary_rows: an output without its rows")
+            args += [None, None]
+            outs.append(None)
+            continue
+        _need(tuple(x.shape[:2]) == (n_seqs, n_new) and x.shape[3] == d and x.device == first.device, "rotary_rows: q and k differ")
+        if out is None:
+            out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        _need(out.shape == x.shape and out.device == x.device, "rotary_rows: out has the rows' shape")
+        args += [_rows(x, "rotary_rows"), _rows(out, "rotary_rows")]
+        outs.append(out)
+    _check(_run_on(first.device, lambda st: lib.yahkv_rotary_apply(
+        C.byref(rotary.struct), d, _dp(positions), n_seqs, n_new, *map(_ref, args), st)), "rotary_apply")
+    return tuple(outs)
+
+
+def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None, q_out=None, q_out_dtype=None, k_out=None,
+                  n_valid=None):
+    """append() with the rotation of k (and of q, if given) fused in: k / v [n_seqs][n_new][n_kv_heads][D] and q
+    [n_seqs][n_new][n_q_heads][D] at any strides of whole 16 bytes, token t of sequence s to slot start_pos[s] + t, turned by
+    positions[s][t] (None: by its slot). k_out (f32, contiguous) also receives the rotated K rows. Returns q_out."""
+    import torch
+    g = pools.geom
+    _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and tuple(k.shape[2:]) == (g.n_kv_heads, g.head_dim),
+          f"rotary_append: k and v [n_seqs][n_new][{g.n_kv_heads}][{g.head_dim}] are expected")
+    n_seqs, n_new = k.shape[:2]
+    dev = pools.kq.device
+    _need(k.device == dev and v.device == dev and rotary.turns.device == dev, "rotary_append: another device than the pools'")
+    _table(table, n_seqs, dev, "page table")
+    _ints(start_pos, (n_seqs,), dev, "start_pos")
+    if n_valid is not None:
+        _ints(n_valid, (n_seqs,), dev, "n_valid")
+    if positions is not None:
+        _ints(positions, (n_seqs, n_new), dev, "positions")
+    rotary.check_head(g.head_dim)
+    qs = qd = None
+    if q is not None:
+        _need(tuple(q.shape) == (n_seqs, n_new, g.n_q_heads, g.head_dim) and q.dtype == k.dtype and q.device == dev,
+              f"rotary_append: q [n_seqs][n_new][{g.n_q_heads}][{g.head_dim}] of k's type is expected")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q_out_dtype or torch.float32, device=dev)
+        _need(q_out.shape == q.shape and q_out.device == dev, "rotary_append: q_out has q's shape")
+        qs, qd = _rows(q, "q"), _rows(q_out, "q_out")
+    _need(q is not None or q_out is None, "rotary_append: q_out without q")
+    _need(k_out is None or (k_out.dtype == torch.float32 and k_out.is_contiguous() and k_out.shape == k.shape and
+                            k_out.device == dev), "rotary_append: k_out is contiguous f32 of k's shape")
+    st, ks, vs = pools.struct(), _rows(k, "k"), _rows(v, "v")
+    _check(_run_on(dev, lambda stream: lib.yahkv_rotary_append(
+        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(start_pos), _dp(n_valid), n_seqs, n_new,
+        C.byref(rotary.struct), _dp(positions), C.byref(ks), C.byref(vs), _ref(qs), _ref(qd), _dp(k_out), stream)),
+        "rotary_append")
+    return q_out
+
+
+def decode_shared_workspace_bytes(g, n_seqs, n_groups, max_shared_len, max_tail_len):
+    return lib.yahkv_decode_shared_workspace_bytes(C.byref(g), n_seqs, n_groups, max_shared_len, max_tail_len)
+
+
+def decode_attend_shared(pools, table, seq_len, group_first, shared_len, max_shared_len, max_tail_len, q, scale, gate=None,
+                         out=None, out_dtype=None, workspace=None):
+    """decode_attend() for a batch that shares prefixes: sequences group_first[j] .. group_first[j + 1] - 1 begin with
+    shared_len[j] common tokens, whose whole 64-token tiles lie in the same pages of all their table rows and are read once.
+    max_shared_len and max_tail_len are host bounds of shared_len and of what a sequence reads besides. Returns out (f32
+    unless out / out_dtype say otherwise)."""
+    import torch
+    g = pools.geom
+    _queries(g, q, gate, pools, "decode_attend_shared")
+    n_seqs, dev = q.shape[0], q.device
+    _table(table, n_seqs, dev, "page table")
+    _ints(seq_len, (n_seqs,), dev, "seq_len")
+    _need(shared_len.dim() == 1, "shared_len: one length per group")
+    n_groups = shared_len.shape[0]
+    _ints(shared_len, (n_groups,), dev, "shared_len")
+    _ints(group_first, (n_groups + 1,), dev, "group_first")
+    out = _out(out, q.shape, out_dtype, dev, torch.float32)
+    workspace = _scratch(workspace, 0 if workspace is not None else decode_shared_workspace_bytes(
+        g, n_seqs, n_groups, max_shared_len, max_tail_len), dev)
+    st = pools.struct()
+    _check(_run_on(dev, lambda stream: lib.yahkv_decode_attend_shared(
+        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(seq_len), n_seqs, _dp(group_first), _dp(shared_len),
+        n_groups, max_shared_len, max_tail_len, _dp(q), _dtype_code(q), scale, _dp(gate), _dp(out), _dtype_code(out),
+        _dp(workspace), workspace.numel(), stream)), "decode_attend_shared")
+    return out
+
+
+def decode_weights_workspace_bytes(g, n_seqs, max_seq_len):
+    return lib.yahkv_decode_weights_workspace_bytes(C.byref(g), n_seqs, max_seq_len)
+
+
+def _weight_rows(w, g, n_seqs, least, device, what):
+    import torch
+    _need(w.dtype == torch.float32 and w.is_contiguous() and w.device == device and w.dim() == 3 and
+          tuple(w.shape[:2]) == (n_seqs, g.n_kv_heads) and w.shape[2] >= least,
+          f"{what}: contiguous f32 [{n_seqs}][{g.n_kv_heads}][at least {least}] on {device} is expected")
+
+
+def decode_attend_weights(pools, table, seq_len, max_seq_len, q, scale, weights_out, weights_in=None, decay=1.0, gate=None,
+                          out=None, out_dtype=None, workspace=None):
+    """decode_attend() that also leaves weights_out[s][h][t] = decay * weights_in[s][h][t] + the softmax weights of key t over
+    kv head h's query heads, f32 [n_seqs][n_kv_heads][>= max_seq_len]; weights_in None: zeros; it may be weights_out.
+    Returns out (f32 unless out / out_dtype say otherwise)."""
+    import torch
+    g = pools.geom
+    _queries(g, q, gate, pools, "decode_attend_weights")
+    n_seqs, dev = q.shape[0], q.device
+    _table(table, n_seqs, dev, "page table")
+    _ints(seq_len, (n_seqs,), dev, "seq_len")
+    _weight_rows(weights_out, g, n_seqs, max_seq_len, dev, "weights_out")
+    _need(weights_in is None or (weights_in.shape == weights_out.shape and weights_in.dtype == torch.float32 and
+                                 weights_in.is_contiguous() and weights_in.device == dev), "weights_in: as weights_out")
+    out = _out(out, q.shape, out_dtype, dev, torch.float32)
+    workspace = _scratch(workspace, 0 if workspace is not None else decode_weights_workspace_bytes(g, n_seqs, max_seq_len), dev)
+    st = pools.struct()
+    _check(_run_on(dev, lambda stream: lib.yahkv_decode_attend_weights(
+        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(seq_len), n_seqs, max_seq_len, _dp(q), _dtype_code(q),
+        scale, _dp(gate), _dp(out), _dtype_code(out), _dp(weights_in), _dp(weights_out), weights_out.shape[2], decay,
+        _dp(workspace), workspace.numel(), stream)), "decode_attend_weights")
+    return out
+
+
+def evict_select(g, seq_len, max_seq_len, weights, budget, sink=0, recent=0, kept=None, n_kept=None):
+    """The positions each kv head keeps of a sequence cut to `budget` tokens: the first `sink`, the last `recent`, and of the
+    others the heaviest (ties: the lowest). Returns (kept int32 [n_seqs][n_kv_heads][budget], rising, -1 behind the last;
+    n_kept int32 [n_seqs])."""
+    import torch
+    _need(seq_len.dim() == 1 and seq_len.is_cuda, "seq_len: lengths on the GPU")
+    n_seqs, dev = seq_len.shape[0], seq_len.device
+    _ints(seq_len, (n_seqs,), dev, "seq_len")
+    _weight_rows(weights, g, n_seqs, max_seq_len, dev, "weights")
+    if kept is None:
+        kept = torch.empty((n_seqs, g.n_kv_heads, max(budget, 0)), dtype=torch.int32, device=dev)
+    if n_kept is None:
+        n_kept = torch.empty(n_seqs, dtype=torch.int32, device=dev)
+    _ints(kept, (n_seqs, g.n_kv_heads, max(budget, 0)), dev, "kept")
+    _ints(n_kept, (n_seqs,), dev, "n_kept")
+    _check(_run_on(dev, lambda stream: lib.yahkv_evict_select(
+        C.byref(g), _dp(seq_len), n_seqs, max_seq_len, _dp(weights), weights.shape[2], budget, sink, recent, _dp(kept),
+        _dp(n_kept), stream)), "evict_select")
+    return kept, n_kept
+
+
+def evict_compact(pools, table, kept, n_kept, dst_table, weights_in=None, weights_out=None):
+    """Moves the kept tokens (evict_select's) of every sequence to slots 0 .. n_kept[s] - 1 of the new pages dst_table[s], bit
+    for bit, and their weights along. The new pages must not be among the sequences' present ones."""
+    g = pools.geom
+    dev = pools.kq.device
+    _need(kept.dim() == 3 and kept.shape[0] > 0 and kept.shape[2] > 0, "kept: [n_seqs][n_kv_heads][budget]")
+    n_seqs, budget = kept.shape[0], kept.shape[2]
+    _ints(kept, (n_seqs, g.n_kv_heads, budget), dev, "kept")
+    _ints(n_kept, (n_seqs,), dev, "n_kept")
+    _table(table, n_seqs, dev, "page table")
+    _table(dst_table, n_seqs, dev, "dst_table")
+    if weights_in is not None:
+        _weight_rows(weights_in, g, n_seqs, 1, dev, "weights_in")
+    if weights_out is not None:
+        _weight_rows(weights_out, g, n_seqs, budget, dev, "weights_out")
+    st = pools.struct()
+    _check(_run_on(dev, lambda stream: lib.yahkv_evict_compact(
+        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(kept), _dp(n_kept), n_seqs, budget, _dp(dst_table),
+        dst_table.shape[1], _dp(weights_in), 0 if weights_in is None else weights_in.shape[2], _dp(weights_out),
+        0 if weights_out is None else weights_out.shape[2], stream)), "evict_compact")
 
 
 # ---- kv8a16: the reference's own KV format (yahkv_kv8_*) --------------------------------------------------------------

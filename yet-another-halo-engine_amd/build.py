@@ -6,7 +6,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libyahkv.so")
-SOURCES = ["host.cpp", "append.hip", "decode.hip", "prefill.hip", "slots.hip", "f16kv.hip", "kv8_append.hip",
+SOURCES = ["host.cpp", "append.hip", "rotary.hip", "evict.hip", "decode.hip", "shared.hip", "prefill.hip", "slots.hip", "f16kv.hip", "kv8_append.hip",
            "kv8_decode.hip", "refslot.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra",

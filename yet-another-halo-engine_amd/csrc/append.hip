@@ -11,11 +11,14 @@
 //   inv_rms = rsqrt(sum_i x[i]^2 / head_dim + eps); normed[i] = (x[i] * inv_rms) * weight[i]
 //   angle(p) = pos * (1 / theta^(2 p / rotary_dim)), p < half = rotary_dim / 2
 //   out[p] = normed[p] cos - normed[p + half] sin; out[p + half] = normed[p] sin + normed[p + half] cos
-// and dims at or past rotary_dim are only normalised. The angle uses the token's position as given; the page slot
+// and dims at or past rotary_dim are only normalised (yahkv_rotary_append: rotary.hpp's angles, either layout, a part of
+// the head, positions and row strides of their own, the norm optional). The angle uses the token's position as given; the page slot
 // uses the position clamped to the table, as in the reference (:89-94). What the reference stores as f16 rows is
 // stored here as q8_0 / q4_0 blocks: the rotated K never makes a round trip through memory as f32.
 #include "common.hpp"
 #include "quant.hpp"
+#include "rotary.hpp"
+#include "store.hpp"
 
 namespace yahkv {
 namespace {
@@ -42,25 +45,13 @@ struct RopeArgs {
   int32_t per_xcd;    // AppendRows: tokens per XCD and sequence (a multiple of the page), or 0: tokens in order
   int32_t skip_v;     // AppendRows: the V rows are left to another launch (AppendPages with skip_k)
   int32_t skip_k;     // AppendPages: V only
+  // yahkv_rotary_append (kGeneral rows): the rotation, positions of its own (or null), and rows at strides of their own
+  RotaryArgs rotary;
+  const int32_t* positions;
+  RowsArgs k_rows, v_rows, q_rows, q_out_rows;
 };
-
-__device__ __forceinline__ void Store4(void* dst, size_t i, int dtype, float4 v) {
-  if (dtype == YAHKV_F32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(dst) + i) = v;
-    return;
-  }
-  uint32_t lo, hi;
-  if (dtype == YAHKV_F16) {
-    typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-    lo = __builtin_bit_cast(uint32_t, h2v{static_cast<_Float16>(v.x), static_cast<_Float16>(v.y)});
-    hi = __builtin_bit_cast(uint32_t, h2v{static_cast<_Float16>(v.z), static_cast<_Float16>(v.w)});
-  } else {
-    typedef __bf16 b2v __attribute__((ext_vector_type(2)));
-    lo = __builtin_bit_cast(uint32_t, b2v{static_cast<__bf16>(v.x), static_cast<__bf16>(v.y)});
-    hi = __builtin_bit_cast(uint32_t, b2v{static_cast<__bf16>(v.z), static_cast<__bf16>(v.w)});
-  }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + i) = uint2{lo, hi};
-}
+// What AppendRows does to K and query rows before it stores them.
+enum RowsMode { kAsTheyAre = 0, kNeox = 1, kGeneral = 2 };
 
 // One workgroup of four wavefronts per token. With ROPE, the token's angles (they depend on the position and the
 // pair, not on the head) are computed once into LDS; without, K rows are quantized as they are (plain append) and
@@ -72,9 +63,10 @@ __device__ __forceinline__ void Store4(void* dst, size_t i, int dtype, float4 v)
 // branches, so the source rows' type SRC is known when compiling (as in AppendPages: with the type a run-time value
 // each load waited for the one before) and a row or lane that has nothing to load asks for an address that exists.
 constexpr int kRopeWaves = 4, kRowsInFlight = 8;
-template <int FMT, bool ROPE, int SRC>
+template <int FMT, int MODE, int SRC>
 __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) {
 #pragma clang fp contract(off)
+  constexpr bool ROPE = MODE != kAsTheyAre;
   const Geom g = a.g;
   const int H = g.n_kv, PT = g.pt, D = g.hd, NQ = a.q_src != nullptr ? g.n_q : 0;
   // (with a.skip_v the token's rows are its K heads and its query heads: row numbers H .. 2 H - 1 are passed over)
@@ -104,7 +96,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) 
   __shared__ __align__(16) float cs[128], sn[128];  // rotary_dim / 2 <= 128
   const int rot = a.rotary_dim, half = rot / 2;
   const float posf = static_cast<float>(pos_raw);
-  if (ROPE) {
+  if constexpr (MODE == kNeox) {
     for (int p = threadIdx.x; p < half; p += 64 * kRopeWaves) {
       const float inv_freq = 1.0f / powf(a.theta, (2.0f * static_cast<float>(p)) / static_cast<float>(rot));
       float sv, cv;
@@ -113,22 +105,35 @@ __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) 
     }
     __syncthreads();
   }
+  if constexpr (MODE == kGeneral) {
+    const int turn_pos = a.positions != nullptr ? a.positions[int64_t(s) * a.n_new + i] : pos_raw;
+    for (int p = threadIdx.x; p < half; p += 64 * kRopeWaves) {
+      float cv, sv;
+      TurnCosSin(turn_pos, a.rotary.turns[p], &cv, &sv);
+      cs[p] = cv * a.rotary.magnitude, sn[p] = sv * a.rotary.magnitude;
+    }
+    __syncthreads();
+  }
   const int d0 = 4 * lane;  // this lane's four dims of every row
   const bool has = d0 < D;
   // This lane's part of the rotation, the same for every row: element e = d0 + j is the first of its pair
   // (e < half: out = x c - partner s, partner = e + half), the second (half <= e < rot: out = partner s + x c,
   // partner = e - half) or past the rotated dims. rotary_dim / 2 is a multiple of 4 (checked by the entry point), so
-  // the four partners lie in one lane.
+  // the four partners lie in one lane. (The general rotation counts from its first dim, a multiple of 4; in its
+  // interleaved layout a lane holds two whole pairs.)
   float c4[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   int partner_lane = lane;
-  if (ROPE && has && d0 < rot) {
-    const bool first = d0 < half;
-    partner_lane = first ? lane + half / 4 : lane - half / 4;
+  const int r0 = MODE == kGeneral ? d0 - a.rotary.first : d0;
+  const bool pairs_inside = MODE == kGeneral && a.rotary.layout == YAHKV_ROTARY_INTERLEAVED;
+  const bool turned = ROPE && has && r0 >= 0 && r0 < rot;
+  if (turned) {
+    const bool first = r0 < half;
+    if (!pairs_inside) partner_lane = first ? lane + half / 4 : lane - half / 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = first ? d0 + j : d0 + j - half;
+      const int p = pairs_inside ? (r0 + j) / 2 : first ? r0 + j : r0 + j - half;
       c4[j] = cs[p];
-      s4[j] = first ? -sn[p] : sn[p];
+      s4[j] = (pairs_inside ? j % 2 == 0 : first) ? -sn[p] : sn[p];
     }
   }
   float4 wk = {1.0f, 1.0f, 1.0f, 1.0f}, wq = wk;  // this lane's norm weights
@@ -136,6 +141,12 @@ __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) 
   if (ROPE && a.q_weight != nullptr && has) wq = *reinterpret_cast<const float4*>(a.q_weight + d0);
   // source of row `row` of the token and its element offset
   auto source = [&](int row, const void** src, size_t* off) {
+    if constexpr (MODE == kGeneral) {
+      const RowsArgs& r = row < H ? a.k_rows : row < 2 * H ? a.v_rows : a.q_rows;
+      *src = r.data;
+      *off = static_cast<size_t>(s * r.seq + i * r.token + (row < H ? row : row < 2 * H ? row - H : row - 2 * H) * r.head);
+      return;
+    }
     const size_t tok = size_t(s) * a.n_new + i;
     if (row < H) *src = a.k_src, *off = (tok * H + row) * D;
     else if (row < 2 * H) *src = a.v_src, *off = (tok * H + (row - H)) * D;
@@ -158,23 +169,32 @@ __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) 
       float4 v = Widen4(raw[j], SRC);
       if (!has) v = float4{0.0f, 0.0f, 0.0f, 0.0f};
       if (ROPE && !is_v) {
-        const float ss = WaveSum(v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w);
-        const float inv_rms = 1.0f / sqrtf(ss / static_cast<float>(D) + a.eps);
-        const float4 w = is_q ? wq : wk;
-        v = float4{(v.x * inv_rms) * w.x, (v.y * inv_rms) * w.y, (v.z * inv_rms) * w.z, (v.w * inv_rms) * w.w};
-        const float px = __shfl(v.x, partner_lane, 64), py = __shfl(v.y, partner_lane, 64);
-        const float pz = __shfl(v.z, partner_lane, 64), pw = __shfl(v.w, partner_lane, 64);
+        if (MODE == kNeox || a.rotary.normalise) {
+          const float ss = WaveSum(v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w);
+          const float inv_rms = 1.0f / sqrtf(ss / static_cast<float>(D) + a.eps);
+          const float4 w = is_q ? wq : wk;
+          v = float4{(v.x * inv_rms) * w.x, (v.y * inv_rms) * w.y, (v.z * inv_rms) * w.z, (v.w * inv_rms) * w.w};
+        }
+        float px, py, pz, pw;
+        if (pairs_inside) {
+          px = v.y, py = v.x, pz = v.w, pw = v.z;
+        } else {
+          px = __shfl(v.x, partner_lane, 64), py = __shfl(v.y, partner_lane, 64);
+          pz = __shfl(v.z, partner_lane, 64), pw = __shfl(v.w, partner_lane, 64);
+        }
         // first of a pair: x c - partner s; second: partner s + x c (s4 carries the sign); past rot: c = 1, s = 0
-        v = float4{v.x * c4[0] + px * s4[0], v.y * c4[1] + py * s4[1], v.z * c4[2] + pz * s4[2],
-                   v.w * c4[3] + pw * s4[3]};
+        if (MODE == kNeox || turned)
+          v = float4{v.x * c4[0] + px * s4[0], v.y * c4[1] + py * s4[1], v.z * c4[2] + pz * s4[2], v.w * c4[3] + pw * s4[3]};
       }
       const void* src;
       size_t off;
       source(row, &src, &off);
       if (is_q) {
+        if constexpr (MODE == kGeneral) off = static_cast<size_t>(s * a.q_out_rows.seq + i * a.q_out_rows.token + (row - 2 * H) * a.q_out_rows.head);
         if (has) Store4(a.q_out, off + d0, a.q_out_dtype, v);
         continue;
       }
+      if constexpr (MODE == kGeneral) off = ((size_t(s) * a.n_new + i) * H + row) * D;  // of k_out, for the K rows
       if (!is_v && a.k_out != nullptr && has) *reinterpret_cast<float4*>(a.k_out + off + d0) = v;
       // quantize: block b = lanes 8 b .. 8 b + 7
       const int h = is_v ? row - H : row, lb = lane % 8;
@@ -239,9 +259,9 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
       const int t = 4 * q + j;
       rk[j] = rv[j] = uint4{0u, 0u, 0u, 0u};  // reads as 0.0 in every source type
       if (t >= t_lo && t < t_hi && has) {
-        const size_t row = ((size_t(s) * a.n_new + token_at(pi * PT + t)) * H + h) * D;
-        rv[j] = LoadRaw4(a.v_src, row + d0, SRC);
-        if (!a.skip_k) rk[j] = LoadRaw4(a.k_src, row + d0, SRC);
+        const int tok = token_at(pi * PT + t);
+        rv[j] = LoadRaw4(a.v_src, static_cast<size_t>(s * a.v_rows.seq + tok * a.v_rows.token + h * a.v_rows.head) + d0, SRC);
+        if (!a.skip_k) rk[j] = LoadRaw4(a.k_src, ((size_t(s) * a.n_new + tok) * H + h) * D + d0, SRC);
       }
     }
   };
@@ -416,7 +436,7 @@ void LaunchPages(int32_t format, int32_t src_dtype, int32_t n_seqs, int32_t n_ne
     else hipLaunchKernelGGL((AppendPages<4, YAHKV_BF16>), grid, block, 0, st, a);
   }
 }
-template <bool ROPE>
+template <int ROPE>
 void LaunchRows(int32_t format, int32_t src_dtype, dim3 grid, hipStream_t st, const RopeArgs& a) {
   const dim3 block(64 * kRopeWaves);
   if (format == YAHKV_Q8_0) {
@@ -428,6 +448,36 @@ void LaunchRows(int32_t format, int32_t src_dtype, dim3 grid, hipStream_t st, co
     else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_F16>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_BF16>), grid, block, 0, st, a);
   }
+}
+// Rows [n_seqs][n_new][n_kv][D] without gaps.
+RowsArgs DenseRows(const RopeArgs& a, const void* data) {
+  const int64_t token = int64_t(a.g.n_kv) * a.g.hd;
+  return RowsArgs{const_cast<void*>(data), a.src_dtype, a.g.n_kv, token * a.n_new, token, a.g.hd};
+}
+// The fused forms: K and query rows turned, V as it is.
+template <int MODE>
+int LaunchTurned(RopeArgs a, hipStream_t st) {
+  const Geom& m = a.g;
+  const int n_seqs = a.n_seqs, n_new = a.n_new, format = a.g.format, src_dtype = a.src_dtype;
+  const int64_t tokens = int64_t(n_seqs) * n_new;
+  if (tokens > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
+  if (n_new >= kPageAppendMin && n_seqs <= 65535) {
+    // A chunk: V page by page, as the plain append takes it (whole lines from an image of the page, where the
+    // token's workgroup would store V's codes byte by byte into the transposed page), K and the query rows by token.
+    RopeArgs v = a;
+    v.skip_k = 1;
+    LaunchPages(format, src_dtype, n_seqs, n_new, st, v);
+    if (const int rc = LaunchStatus()) return rc;
+    a.skip_v = 1;
+  }
+  int64_t blocks = tokens;
+  if (n_new >= 8 * m.pt) {  // a long chunk: a page's tokens to one XCD (see AppendRows)
+    a.per_xcd = ((n_new + 7) / 8 + m.pt - 1) / m.pt * m.pt;
+    blocks = int64_t(n_seqs) * 8 * a.per_xcd;
+    if (blocks > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
+  }
+  LaunchRows<MODE>(format, src_dtype, dim3(static_cast<unsigned>(blocks)), st, a);
+  return LaunchStatus();
 }
 }  // namespace
 
@@ -441,14 +491,14 @@ extern "C" int yahkv_append(const yahkv_geometry* g, const yahkv_pools* pools, c
   RopeArgs a{};
   a.g = MakeGeom(*g), a.pools = MakePools(*pools), a.table = page_table, a.stride = page_table_stride;
   a.start_pos = start_pos, a.n_valid = n_valid, a.n_seqs = n_seqs, a.n_new = n_new, a.k_src = k_src, a.v_src = v_src;
-  a.src_dtype = src_dtype, a.rotary_dim = 8, a.theta = 1.0f;
+  a.src_dtype = src_dtype, a.rotary_dim = 8, a.theta = 1.0f, a.v_rows = DenseRows(a, v_src);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (n_new >= kPageAppendMin && n_seqs <= 65535) {  // a chunk: page by page (the grid's z extent is the batch)
     LaunchPages(g->format, src_dtype, n_seqs, n_new, st, a);
     return LaunchStatus();
   }
   const dim3 grid(static_cast<unsigned>(n_seqs) * static_cast<unsigned>(n_new));
-  LaunchRows<false>(g->format, src_dtype, grid, st, a);
+  LaunchRows<kAsTheyAre>(g->format, src_dtype, grid, st, a);
   return LaunchStatus();
 }
 
@@ -472,26 +522,35 @@ extern "C" int yahkv_append_rope(const yahkv_geometry* g, const yahkv_pools* poo
   a.n_valid = n_valid, a.n_seqs = n_seqs, a.n_new = n_new, a.k_src = k_src, a.v_src = v_src, a.src_dtype = src_dtype;
   a.k_weight = rope->k_weight, a.q_weight = rope->q_weight, a.theta = rope->theta, a.eps = rope->eps;
   a.rotary_dim = rope->rotary_dim, a.q_src = q_src, a.q_out = q_out, a.q_out_dtype = q_out_dtype, a.k_out = k_out;
-  const int64_t tokens = int64_t(n_seqs) * n_new;
-  if (tokens > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  if (n_new >= kPageAppendMin && n_seqs <= 65535) {
-    // A chunk: V page by page, as the plain append takes it (whole lines from an image of the page, where the
-    // token's workgroup would store V's codes byte by byte into the transposed page), K and the query rows by token.
-    RopeArgs v = a;
-    v.skip_k = 1;
-    LaunchPages(g->format, src_dtype, n_seqs, n_new, st, v);
-    if (const int rc = LaunchStatus()) return rc;
-    a.skip_v = 1;
+  a.v_rows = DenseRows(a, v_src);
+  return LaunchTurned<kNeox>(a, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
+                                   int32_t page_table_stride, const int32_t* start_pos, const int32_t* n_valid,
+                                   int32_t n_seqs, int32_t n_new, const yahkv_rotary* rotary, const int32_t* positions,
+                                   const yahkv_rows* k, const yahkv_rows* v, const yahkv_rows* q_src,
+                                   const yahkv_rows* q_dst, float* k_out, void* stream) {
+  if (k == nullptr || v == nullptr) return YAHKV_ERR_ARG;
+  if (const int st = CheckAppend(g, pools, page_table, page_table_stride, start_pos, n_seqs, n_new, k->data, v->data, k->dtype))
+    return st;
+  RopeArgs a{};
+  a.g = MakeGeom(*g), a.pools = MakePools(*pools), a.table = page_table, a.stride = page_table_stride;
+  if (const int st = CheckRotary(rotary, a.g.hd, &a.rotary)) return st;
+  if (const int st = CheckRows(k, &a.k_rows)) return st;
+  if (const int st = CheckRows(v, &a.v_rows)) return st;
+  if (k->n_heads != g->n_kv_heads || v->n_heads != g->n_kv_heads || v->dtype != k->dtype) return YAHKV_ERR_ARG;
+  if ((q_src == nullptr) != (q_dst == nullptr) || !Aligned16(k_out)) return YAHKV_ERR_ARG;
+  if (q_src != nullptr) {
+    if (const int st = CheckRows(q_src, &a.q_rows)) return st;
+    if (const int st = CheckRows(q_dst, &a.q_out_rows)) return st;
+    if (q_src->n_heads != g->n_q_heads || q_dst->n_heads != g->n_q_heads || q_src->dtype != k->dtype) return YAHKV_ERR_ARG;
+    a.q_src = q_src->data, a.q_out = q_dst->data, a.q_out_dtype = q_dst->dtype;
   }
-  int64_t blocks = tokens;
-  if (n_new >= 8 * m.pt) {  // a long chunk: a page's tokens to one XCD (see AppendRows)
-    a.per_xcd = ((n_new + 7) / 8 + m.pt - 1) / m.pt * m.pt;
-    blocks = int64_t(n_seqs) * 8 * a.per_xcd;
-    if (blocks > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
-  }
-  LaunchRows<true>(g->format, src_dtype, dim3(static_cast<unsigned>(blocks)), st, a);
-  return LaunchStatus();
+  a.start_pos = start_pos, a.n_valid = n_valid, a.n_seqs = n_seqs, a.n_new = n_new, a.src_dtype = k->dtype;
+  a.k_src = k->data, a.v_src = v->data, a.k_out = k_out, a.positions = positions;
+  a.rotary_dim = a.rotary.rot, a.eps = a.rotary.eps, a.k_weight = a.rotary.k_weight, a.q_weight = a.rotary.q_weight;
+  return LaunchTurned<kGeneral>(a, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int yahkv_gather_blocks(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* table_row,

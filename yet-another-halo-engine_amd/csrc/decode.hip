@@ -23,9 +23,11 @@
 #include <mutex>
 #include <vector>
 
+#include "codes.hpp"
 #include "common.hpp"
 #include "decode_cut.hpp"
 #include "quant.hpp"
+#include "store.hpp"
 
 namespace yahkv {
 namespace {
@@ -47,39 +49,6 @@ namespace {
 // [key][32]) or 16 keys of one dim (V^T, [dim][key]). q4_0: a lane's 8-byte K load is half a block of one key (low
 // nibbles dims 8 h + 0..7, high nibbles dims 16 + 8 h + 0..7, [block][key][16]); its 16-byte V load is 16 keys of the
 // byte row that holds dims j and j + 16 of a block ([block][16][key]), which feeds two 16-dim output tiles.
-
-// Eight int8 codes (two dwords) as eight f16, exact. 0x6400 | u is the f16 1024 + u; u = code + 128.
-__device__ __forceinline__ h8v Codes8(uint32_t w0, uint32_t w1) {
-  const h2v off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
-  const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u;
-  const h2v a = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u)) + off;
-  const h2v b = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u)) + off;
-  const h2v c = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u)) + off;
-  const h2v d = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u)) + off;
-  return h8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// Eight nibbles of two dwords as eight f16 holding (nibble - 8), exact. Low nibbles: 0x6400 | n is 1024 + n. High
-// nibbles stay in place: 0x6400 | (n << 4) is 1024 + 16 n, and one fused multiply-add takes it to n - 8.
-__device__ __forceinline__ h8v NibblesLo8(uint32_t w0, uint32_t w1) {
-  const h2v off = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
-  const uint32_t x0 = w0 & 0x0F0F0F0Fu, x1 = w1 & 0x0F0F0F0Fu;
-  const h2v a = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u)) + off;
-  const h2v b = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u)) + off;
-  const h2v c = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u)) + off;
-  const h2v d = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u)) + off;
-  return h8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-__device__ __forceinline__ h8v NibblesHi8(uint32_t w0, uint32_t w1) {
-  const h2v mul = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-  const h2v off = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
-  const uint32_t x0 = w0 & 0xF0F0F0F0u, x1 = w1 & 0xF0F0F0F0u;
-  const h2v a = __builtin_elementwise_fma(__builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u)), mul, off);
-  const h2v b = __builtin_elementwise_fma(__builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u)), mul, off);
-  const h2v c = __builtin_elementwise_fma(__builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u)), mul, off);
-  const h2v d = __builtin_elementwise_fma(__builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u)), mul, off);
-  return h8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // The same without the subtraction, for the first product: 1024 + 128 + code (q8_0), 1024 + nibble (low nibbles),
 // 1024 + 16 * nibble (high nibbles, in place). What the constants add to a score depends on the queries alone and is
@@ -134,7 +103,10 @@ __device__ __forceinline__ int Arrive(unsigned long long* ticket, uint32_t n) {
 // MODE 2: two dispatches as MODE 0, but what the waves have of the chunk's LAST pair meets in LDS and leaves as one
 // partial instead of eight (the in-LDS merge of the one-launch form, without its tickets). For a small batch, where a
 // chunk is a few tiles of a single pair, that is an eighth of the partials to write here and to read in the merge.
-template <int FMT, int D, int PT, int MODE>
+// WEIGH: the scores also go to memory (DecodeArgs::scores), and they are those of the codes alone: the constants of the
+// codes' f16 conversion are subtracted before the product, not after it, which leaves sums of exact products of the
+// values' own size (the other form's 1e-5 of a score would be a relative error of that size in every weight).
+template <int FMT, int D, int PT, int MODE, bool WEIGH = false>
 __global__ __launch_bounds__(64 * kWavesPerGroup) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void DattnPart(const DecodeArgs a) {
   constexpr bool FUSED = MODE == 1, HOLD = MODE != 0;
@@ -349,6 +321,10 @@ void DattnPart(const DecodeArgs a) {
   };
   // the 8 codes of block b this lane feeds to instruction `sub` of the block's pair
   auto kcodes = [&](int b, int sub) -> h8v {
+    if constexpr (WEIGH) {
+      if constexpr (Q8) return Codes8(kb[b][2 * sub], kb[b][2 * sub + 1]);
+      return sub == 0 ? NibblesLo8(kb[b][0], kb[b][1]) : NibblesHi8(kb[b][0], kb[b][1]);
+    }
     if constexpr (Q8) return RawCodes8(kb[b][2 * sub], kb[b][2 * sub + 1]);
     return sub == 0 ? RawNibbles8<0x0F0F0F0Fu>(kb[b][0], kb[b][1]) : RawNibbles8<0xF0F0F0F0u>(kb[b][0], kb[b][1]);
   };
@@ -487,11 +463,11 @@ void DattnPart(const DecodeArgs a) {
       float t = 0.0f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) t += static_cast<float>(qreg[e][k]);
-      t *= Q8 ? 1152.0f : (sub == 0 ? 1032.0f : 72.0f);
+      t *= WEIGH ? 0.0f : Q8 ? 1152.0f : (sub == 0 ? 1032.0f : 72.0f);
       t += __shfl_xor(t, 8, 64);
       t += __shfl_xor(t, 16, 64);
       if (lane % 32 < 8) lcorr[i / 32][i % 8] = t;
-      if constexpr (!Q8) {
+      if constexpr (!Q8 && !WEIGH) {
         if (sub == 1) qreg[e] *= static_cast<_Float16>(0.0625f);  // high nibbles come as 16 n
       }
       *reinterpret_cast<h8v*>(&lq[i / 32][sub][(i / 8) % 2][i % 8][0]) = qreg[e];
@@ -529,7 +505,14 @@ void DattnPart(const DecodeArgs a) {
       for (int tt = 0; tt < 2; ++tt) {
         const bool valid = tile * kTile + 32 * tt + n32 < cur.len;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[tt][r] = valid ? sc[tt][r] : kNegMax;
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (WEIGH) {
+            const int row = 4 * half + r;
+            if (valid && row < G)
+              a.scores[(size_t(cur.s) * g.n_q + size_t(head) * G + row) * a.score_stride + tile * kTile + 32 * tt + n32] = sc[tt][r];
+          }
+          sc[tt][r] = valid ? sc[tt][r] : kNegMax;
+        }
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -1194,7 +1177,7 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
   if (p0 + t < p1) first_ml = *reinterpret_cast<const float2*>(&a.ml[((p0 + t) * G + gi) * 2]);
   if (stores_new && t < 128) StepToken(a, rows, s, h, hq, t / 64, t % 64, gi == 0 && blockIdx.z == 0, &new_score, new_v);
   if (ts <= 0 && !has_new) {  // nothing to attend to
-    for (int d = t; d < DZ; d += RT) a.out[o + d] = 0.0f;
+    for (int d = t; d < DZ; d += RT) Store1(a.out, o + d, a.out_dtype, 0.0f);
     return;
   }
   constexpr int NW = RT / 64;
@@ -1265,8 +1248,49 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
     }
     v /= lt;
     if (a.gate != nullptr) v *= 1.0f / (1.0f + __expf(-a.gate[o + d]));
-    a.out[o + d] = v;
+    Store1(a.out, o + d, a.out_dtype, v);
+    if (a.row_ml != nullptr && d == 0 && d0 == 0) {
+      float* ml = a.row_ml + (size_t(s) * g.n_q + hq) * 2;
+      ml[0] = M, ml[1] = lt;
+    }
   }
+}
+
+// ---- the weights --------------------------------------------------------------------------------------------------------
+
+// weights_out[s][h][t] = decay * weights_in[s][h][t] + sum over the head's query rows of e^(score - M) / l: a thread per
+// key, the rows' maxima and sums the same for a workgroup. Reads 4 G + 4 and writes 4 bytes a key, a tenth of what the
+// key's K and V rows take.
+struct WeighArgs {
+  const int32_t* seq_len;
+  const float* scores;
+  const float* row_ml;
+  const float* in;
+  float* out;
+  int32_t n_q, n_kv, score_stride, stride, max_len;
+  float decay;
+};
+constexpr int kWeighThreads = 256;
+__global__ __launch_bounds__(kWeighThreads) void WeighKeys(const WeighArgs a) {
+  const int h = blockIdx.y, s = blockIdx.z, G = a.n_q / a.n_kv;
+  const int len = min(max(a.seq_len[s], 0), a.max_len);
+  const int t = blockIdx.x * kWeighThreads + threadIdx.x;
+  if (t >= len) return;
+  constexpr float kLog2e = 1.4426950408889634f;
+  const size_t q0 = size_t(s) * a.n_q + size_t(h) * G;
+  float sc[kMaxGroup];
+#pragma unroll
+  for (int r = 0; r < kMaxGroup; ++r) sc[r] = a.scores[(q0 + min(r, G - 1)) * a.score_stride + t];
+  const size_t at = (size_t(s) * a.n_kv + h) * a.stride + t;
+  float w = a.in != nullptr ? a.decay * a.in[at] : 0.0f;
+  float p = 0.0f;
+#pragma unroll
+  for (int r = 0; r < kMaxGroup; ++r) {
+    if (r >= G) break;
+    const float* ml = a.row_ml + (q0 + r) * 2;
+    p += __builtin_amdgcn_exp2f(__builtin_fmaf(-kLog2e, ml[0], sc[r])) / ml[1];
+  }
+  a.out[at] = w + p;
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
@@ -1281,7 +1305,8 @@ int LaunchPart(const DecodeArgs& a, hipStream_t st) {
   }
 #define YAHKV_LAUNCH_PART(FF, DD, PP)                                                                          \
   do {                                                                                                         \
-    if (a.fused) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 1>), grid, dim3(64 * kWavesPerGroup), 0, st, a);           \
+    if (a.scores != nullptr) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 0, true>), grid, dim3(64 * kWavesPerGroup), 0, st, a); \
+    else if (a.fused) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 1>), grid, dim3(64 * kWavesPerGroup), 0, st, a);           \
     else if (a.wg_partials) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 2>), grid, dim3(64 * kWavesPerGroup), 0, st, a); \
     else hipLaunchKernelGGL((DattnPart<FF, DD, PP, 0>), grid, dim3(64 * kWavesPerGroup), 0, st, a);                    \
   } while (0)
@@ -1464,6 +1489,69 @@ extern "C" int yahkv_decode_attend(const yahkv_geometry* g, const yahkv_pools* p
   a.pools = MakePools(*pools), a.table = page_table, a.q = q, a.q_dtype = q_dtype, a.scale = softmax_scale;
   a.gate = gate, a.out = out, a.fused = 1;
   return LaunchPart(a, static_cast<hipStream_t>(stream));
+}
+
+namespace {
+// Two-dispatch form with a partial per wave (the weighing part kernel has no other), and for a batch of few tiles chunks of
+// one tile per wave.
+yahkv_decode_options WeighOptions() {
+  yahkv_decode_options o{};
+  o.wg_partials = 2, o.min_chunk_tiles = kWavesPerGroup;
+  return o;
+}
+struct WeighPlan {
+  size_t part, off_scores, off_ml, bytes;
+  int32_t score_stride;
+};
+WeighPlan MakeWeighPlan(const Geom& m, int32_t n_seqs, int32_t max_seq_len) {
+  const yahkv_decode_options o = WeighOptions();
+  WeighPlan p;
+  p.part = Align(MakePlan(m, n_seqs, max_seq_len, MakeTuning(&o)).bytes);
+  p.score_stride = (max_seq_len + kTile - 1) / kTile * kTile;
+  p.off_ml = p.part;
+  p.off_scores = Align(p.off_ml + sizeof(float) * 2 * size_t(n_seqs) * m.n_q);
+  p.bytes = Align(p.off_scores + sizeof(float) * size_t(n_seqs) * m.n_q * p.score_stride);
+  return p;
+}
+constexpr int32_t kMaxWeighLen = 1 << 30;
+}  // namespace
+
+extern "C" size_t yahkv_decode_weights_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t max_seq_len) {
+  if (CheckGeometry(g) || n_seqs <= 0 || max_seq_len <= 0 || max_seq_len > kMaxWeighLen) return 0;
+  return MakeWeighPlan(MakeGeom(*g), n_seqs, max_seq_len).bytes;
+}
+
+extern "C" int yahkv_decode_attend_weights(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
+                                           int32_t page_table_stride, const int32_t* seq_len, int32_t n_seqs,
+                                           int32_t max_seq_len, const void* q, int32_t q_dtype, float softmax_scale,
+                                           const float* gate, void* out, int32_t out_dtype, const float* weights_in,
+                                           float* weights_out, int32_t weights_stride, float decay, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  if (out == nullptr || (reinterpret_cast<uintptr_t>(out) & 15) || weights_out == nullptr) return YAHKV_ERR_ARG;
+  if (out_dtype != YAHKV_F32 && out_dtype != YAHKV_F16 && out_dtype != YAHKV_BF16) return YAHKV_ERR_ARG;
+  if (const int st = CheckGeometry(g)) return st;
+  if (n_seqs <= 0 || max_seq_len <= 0 || max_seq_len > weights_stride) return YAHKV_ERR_ARG;
+  if (max_seq_len > kMaxWeighLen) return YAHKV_ERR_SHAPE;
+  if (const int st = CheckPartArgs(g, pools, page_table, q, q_dtype)) return st;
+  const Geom m = MakeGeom(*g);
+  const yahkv_decode_options o = WeighOptions();
+  DecodeArgs a;
+  if (const int st = Prepare(m, page_table_stride, seq_len, n_seqs, max_seq_len, workspace, workspace_bytes, &o, &a)) return st;
+  const WeighPlan p = MakeWeighPlan(m, n_seqs, max_seq_len);
+  if (workspace_bytes < p.bytes) return YAHKV_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  a.pools = MakePools(*pools), a.table = page_table, a.q = q, a.q_dtype = q_dtype, a.scale = softmax_scale;
+  a.gate = gate, a.out = static_cast<float*>(out), a.out_dtype = out_dtype;
+  a.scores = reinterpret_cast<float*>(ws + p.off_scores), a.score_stride = p.score_stride;
+  a.row_ml = reinterpret_cast<float*>(ws + p.off_ml);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (const int rc = LaunchPart(a, st)) return rc;
+  if (const int rc = LaunchReduce(a, StepRows{nullptr, nullptr, 0}, &o, st)) return rc;
+  const WeighArgs w{seq_len, a.scores, a.row_ml, weights_in, weights_out, m.n_q, m.n_kv, p.score_stride, weights_stride, a.max_len, decay};
+  const dim3 grid(static_cast<unsigned>((a.max_len + kWeighThreads - 1) / kWeighThreads), static_cast<unsigned>(m.n_kv),
+                  static_cast<unsigned>(n_seqs));
+  hipLaunchKernelGGL(WeighKeys, grid, dim3(kWeighThreads), 0, st, w);
+  return LaunchStatus();
 }
 
 extern "C" int yahkv_decode_calibrate(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,

@@ -59,6 +59,12 @@ struct DecodeArgs {
   // other, so that the waves of a workgroup read a row's heads at the same time. A sequence is then one pair of
   // H x tiles items, item j = (tile j / H, kv head j % H). 0 or 1: the line is cut by (sequence, kv head).
   int32_t tile_mult;
+  int32_t out_dtype;  // of out (yahkv_dtype): F32 for every entry point that has no argument for it
+  // yahkv_decode_attend_weights: the part kernel leaves every key's score (in base-2 units, scale applied), f32
+  // [n_seqs][n_q][score_stride], and the merge every query row's maximum (natural units) and sum, f32 [n_seqs][n_q][2]
+  float* scores;
+  float* row_ml;
+  int32_t score_stride;
 };
 __device__ __forceinline__ int CutHeads(const DecodeArgs& a) { return a.tile_mult > 1 ? 1 : a.g.n_kv; }
 // The step's own token for the reduce kernel: K / V rows [n_seqs][H][D] of `dtype`, or null pointers.
