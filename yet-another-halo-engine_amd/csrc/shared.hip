@@ -3,20 +3,27 @@
 //
 // Attention splits over any partition of the keys: with m a reference point, l = sum 2^(s_t - m) and o = sum 2^(s_t - m)
 // V_t of each part, the whole is (sum 2^(m_p - M) o_p) / (sum 2^(m_p - M) l_p). The prefix's part of a group's rows is a
-// matrix product with many rows (sequences x query heads of a kv head), where the tails, one sequence's query heads each,
-// stay with the split-K kernel of yahkv_decode_part. So: `SharedPart` leaves partials of the prefixes, the decode kernel
-// partials of the tails (from lengths and table rows that begin behind the prefix, which SharedPart writes), `SharedMerge`
-// puts them together.
+// matrix product with many rows (sequences x query heads of a kv head); the tails have one sequence's query heads each.
+// `SharedPart` leaves partials of both in one launch, `SharedMerge` puts them together.
 //
-// SharedPart is the transposed scheme of the prefill kernels (keys along MFMA rows, query rows along lanes):
-//   S^T[key][row] = sum_dim K[key][dim] Q[row][dim]     A = K tile from LDS (16 keys x 32 dims), B = Q^T (registers)
-//   O^T[dim][row] += sum_key V^T[dim][key] P^T[key][row]  A = V^T tile from LDS (16 dims x 32 keys), B = P^T (registers)
-// A workgroup owns RB * WR * 16 query rows of one (group, kv head) and one stretch of the prefix; its 4 waves are WR along
-// the rows and 4 / WR along the keys of a tile. A tile's codes are decoded once per workgroup, into f16 in LDS, by packed
-// f16 arithmetic: perm, add, multiply for two values, the product d * code rounded once.
+// SharedPart: a wave takes 16 RB query rows and 64-key tiles, everything transposed (keys along MFMA rows, query rows along
+// lanes), and works alone: codes go from memory to its registers, are decoded there and feed the products directly.
+//   S^T[key][row] = sum_dim K[key][dim] Q[row][dim]       A = 16 keys x 32 dims, B = Q^T (registers)
+//   O^T[dim][row] += sum_key V^T[dim][key] P^T[key][row]  A = 16 dims x 32 keys, B = P^T (registers)
+// The order of the contraction index is free as long as both operands agree, and so is which key a row of S^T is, so
+// every operand is what a 16-byte load brings: a lane's K load is half a block of one key (q4_0: a block), its V load 16
+// keys of one dim (q4_0: of two). Row i of key tile kt is key 16 (i / 4) + 4 kt + i % 4: then the scores that lane group jg
+// holds after the four key tiles are those of keys 16 jg .. 16 jg + 15, the ones its V load has. P never leaves its lane.
+// A register is asked for again (for the wave's next tile) as soon as its codes are decoded, so a load has about a tile's
+// time to arrive, without a barrier anywhere in the loop. Decoding is packed f16 arithmetic, perm, add, multiply for two
+// values, the product d * code rounded once and saturated at the largest finite f16 (SetSaturation).
+//
+// What bounds it: with 16 or 32 rows the reads; with 48 the vector units (64 decodes of 14 instructions a tile and wave,
+// against 192 matrix instructions of 16 cycles). 48 rows is what fits: accumulators 192, queries 96, codes 128 registers.
 #include "codes.hpp"
 #include "common.hpp"
 #include "decode_cut.hpp"
+#include "quant.hpp"
 #include "store.hpp"
 
 namespace yahkv {
@@ -24,9 +31,10 @@ namespace {
 
 constexpr int kSharedWaves = 4;
 constexpr float kNone = -1.0e30f;  // reference point of a row before its first tile
-// Numerators are 2^(score - m) with m a whole number kBias below the largest score seen: f16 holds them up to 2^kBias and
-// down to 2^-14 - kBias with full precision.
-constexpr float kBias = 10.0f;
+// Numerators are 2^(score - m). m is a whole number, so that moving it rescales exactly, kBias below the largest score when
+// it was set, and is moved when a score exceeds it by kBias + kSlack: numerators stay within f16's range and those
+// 2^-24 of the largest are still normal numbers.
+constexpr float kBias = 10.0f, kSlack = 4.0f;
 
 struct SharedArgs {
   Geom g;
@@ -39,14 +47,12 @@ struct SharedArgs {
   const void* q;
   int32_t q_dtype;
   float scale;
-  int32_t max_blocks, n_split;  // row blocks of all groups at most; pieces a prefix is cut into
-  // workspace
-  int32_t* tail_len;    // [n_seqs]
-  int32_t* tail_table;  // [n_seqs][tail_stride]
-  int32_t tail_stride;
-  float* ml;   // [n_seqs][n_q][slots][2]: reference point (base 2) and sum
-  float* acc;  // [n_seqs][n_q][slots][D]
-  int32_t slots;  // n_split * waves along the keys
+  int32_t max_blocks;           // row blocks of all groups at most
+  int32_t n_split, tail_split;  // pieces a prefix / a tail is cut into
+  int32_t prefix_groups;        // workgroups of the prefixes; those of the tails follow
+  // workspace, [n_seqs][n_q][n_split + tail_split]: reference point (base 2) and sum, accumulator [D]
+  float* ml;
+  float* acc;
 };
 
 __device__ __forceinline__ int GroupFirst(const SharedArgs& a, int j) { return min(max(a.group_first[j], 0), a.n_seqs); }
@@ -63,62 +69,375 @@ __device__ __forceinline__ int GroupOf(const SharedArgs& a, int s) {
   }
   return lo > 0 && s < GroupFirst(a, lo) ? lo - 1 : -1;
 }
-// The keys that a sequence of `len` tokens takes from the prefix of group j: all its whole tiles, or, if it is shorter than
-// they are, none: it is then all tail. So every row of SharedPart sees every key, nothing is masked there, and whatever a
-// prefix holds that a shorter sequence must not see (an infinity would pass through a zero numerator as NaN) stays
-// out of that sequence's sums.
-__device__ __forceinline__ int PrefixOf(const SharedArgs& a, int j, int len) {
-  const int shared = j < 0 ? 0 : GroupShared(a, j);
-  return len < shared ? 0 : shared;
+// What a sequence takes from its group's prefix, all the whole tiles, and from its own row behind them. A sequence that is
+// shorter than those tiles takes none: it is all tail. So every row of a prefix sees every key, nothing is masked there, and
+// whatever a prefix holds that a shorter sequence must not see (an infinity would pass through a zero numerator as NaN)
+// stays out of that sequence's sums.
+struct Keys {
+  int prefix, tail;
+};
+__device__ __forceinline__ Keys KeysOf(const SharedArgs& a, int s) {
+  const int len = min(max(a.seq_len[s], 0), a.stride * a.g.pt), j = GroupOf(a, s);
+  const int shared = j < 0 ? 0 : GroupShared(a, j), prefix = len < shared ? 0 : shared;
+  return Keys{prefix, min(len - prefix, a.max_tail)};
 }
-// A prefix's pieces: tiles per piece, and how many pieces hold any.
-__device__ __forceinline__ int TilesPerPiece(int tiles, int n_split) { return (tiles + n_split - 1) / n_split; }
+// `tiles` cut into at most n pieces: tiles per piece
+__device__ __forceinline__ int PerPiece(int tiles, int n) { return max((tiles + n - 1) / n, 1); }
 
-// Sixteen q8_0 codes times one scale / sixteen scales, or the low or high nibbles of sixteen bytes, as sixteen f16.
-template <int FMT>
-__device__ __forceinline__ void Halves(const uint4 c, int high, h8v* lo, h8v* hi) {
-  if constexpr (FMT == 8) {
-    *lo = Codes8(c.x, c.y), *hi = Codes8(c.z, c.w);
-  } else if (high) {
-    *lo = NibblesHi8(c.x, c.y), *hi = NibblesHi8(c.z, c.w);
-  } else {
-    *lo = NibblesLo8(c.x, c.y), *hi = NibblesLo8(c.z, c.w);
+// Maximum and sum over the four lane groups of a wave (lanes n, n + 16, n + 32, n + 48), in every lane.
+template <typename Op>
+__device__ __forceinline__ float OverLaneGroups(float v, Op op) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  const float w = op(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+  const uint32_t x = __builtin_bit_cast(uint32_t, w);
+  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  const uint32_t q0 = q[0], q1 = q[1];
+  return op(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
+}
+
+// Products d * code beyond the f16 range saturate (they would be infinite, and an infinite score a NaN). MODE.FP16_OVFL
+// (bit 23) does that in the multiply for nothing, but while it is set the matrix unit drops NaN operands, so it is set for
+// the tiles that need it alone: those with a scale above 511 (128 x 511 is below the largest f16) and none that is not
+// finite. k, v: the tile's scales, eight and eight a lane.
+__device__ __forceinline__ void SetSaturation(const uint4 k, const uint4 v) {
+  typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+  auto mag = [](uint32_t w) { return __builtin_bit_cast(u2, w & 0x7FFF7FFFu); };
+  u2 x = __builtin_elementwise_max(mag(k.x), mag(v.x));
+  x = __builtin_elementwise_max(x, __builtin_elementwise_max(mag(k.y), mag(v.y)));
+  x = __builtin_elementwise_max(x, __builtin_elementwise_max(mag(k.z), mag(v.z)));
+  x = __builtin_elementwise_max(x, __builtin_elementwise_max(mag(k.w), mag(v.w)));
+  const uint32_t most = x[0] > x[1] ? x[0] : x[1];
+  const bool large = __builtin_amdgcn_ballot_w64(most > 0x5FFCu) != 0, finite = __builtin_amdgcn_ballot_w64(most >= 0x7C00u) == 0;
+  __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, __builtin_amdgcn_readfirstlane(large && finite ? 1 : 0));
+}
+
+template <int D>
+struct WaveScales {  // a tile's scales in LDS, [key][block] and [block][key]
+  _Float16 k[kTile * D / 32], v[D / 32 * kTile];
+};
+
+// Tiles tile0, tile0 + step, .. below tile1 of the sequence behind table row `row`, from key `origin` on, `n_keys` keys in
+// all (those at or past it are masked), against RB row blocks (query rows prow[]): reference points, this lane's part of the
+// sums, accumulators.
+template <int FMT, int D, int PT, int RB>
+__device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* row, int origin, int h, int tile0, int step,
+                                           int tile1, int n_keys, const size_t (&prow)[RB], WaveScales<D>& lds, float (&m)[RB],
+                                           float (&l)[RB], f4v (&o)[RB][D / 16]) {
+  constexpr int NB = D / 32, NDT = D / 16, KS = D / 32, PPT = kTile / PT;
+  constexpr bool Q8 = FMT == 8;
+  constexpr int NP = Q8 ? KS / 2 : NB / 4;  // K loads per key tile
+  constexpr int SP = KS / NP;               // steps of the first product per K load
+  constexpr int NV = Q8 ? NDT : NB;         // V loads
+  const Geom& g = a.g;
+  const int H = g.n_kv, lane = threadIdx.x % 64, qn = lane % 16, jg = lane / 16;
+  // dims of step (p, sub) that this lane group holds
+  auto dims = [&](int p, int sub) -> int {
+    return Q8 ? 32 * (2 * p + (jg >> 1)) + 16 * (jg & 1) + 8 * sub : 32 * (4 * p + jg) + 8 * (sub & 1) + 16 * (sub >> 1);
+  };
+  h8v qb[RB][KS];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    m[i] = kNone, l[i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qb[i][ks] = LoadQ8(a.q, prow[i] * D + dims(ks / SP, ks % SP), a.q_dtype);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[i][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  if (tile0 >= tile1) return;
+  const float sscale = a.scale * 1.4426950408889634f;
+
+  // pages of a tile, through the constant address space (scalar loads, which the vector memory counter does not see)
+  typedef const int32_t __attribute__((address_space(4))) * ConstRow;
+  const ConstRow crow = (ConstRow)(reinterpret_cast<uintptr_t>(row + origin / PT));
+  const int last_page = a.stride - 1 - origin / PT;
+  auto load_pages = [&](int tile, int (&pg)[PPT]) {
+#pragma unroll
+    for (int j = 0; j < PPT; ++j) pg[j] = ClampPage(crow[min(tile * PPT + j, last_page)], g.n_pages);
+  };
+  auto page_head = [&](const int (&pg)[PPT], int key) -> size_t {  // (page, kv head) of a key of the tile
+    int p = pg[0];
+#pragma unroll
+    for (int j = 1; j < PPT; ++j) p = key / PT == j ? pg[j] : p;
+    return size_t(p) * H + h;
+  };
+  // codes on their way in. Where accumulators and queries leave room, K and V have registers of their own and a load about
+  // a tile's time to arrive; else (three row blocks of 256 dims) they share one set: a V load goes out as soon as a K
+  // load's codes are decoded, and the next tile's K loads as V's are.
+  constexpr bool kOneSet = RB * D > 2 * 256;
+  constexpr int NK = 4 * NP;
+  static_assert(!kOneSet || NK == NV, "a V load for every K load");
+  uint4 kset[NK], vset[kOneSet ? 1 : NV], ksr, vsr;
+  auto kc = [&](int j) -> uint4& { return kset[j]; };
+  auto vc = [&](int j) -> uint4& {
+    if constexpr (kOneSet) return kset[j];
+    else return vset[j];
+  };
+  constexpr uint32_t KB = Q8 ? 32 : 16;
+  // Where a tile is one page, through a buffer resource of the (page, kv head) region: scalar base and offsets, one lane
+  // offset for all loads. Codes that several row blocks read are left to the caches, others go by the non-temporal hint.
+  constexpr int kHint = RB == 3 ? 0 : kStreamed;
+  auto read = [&](const uint8_t* base, uint32_t lane_off, uint32_t off) -> uint4 {
+    if constexpr (PPT == 1) {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7fffffff, 0x00020000);
+      return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, off, kHint));
+    } else {
+      const uint4* at = reinterpret_cast<const uint4*>(base + lane_off + off);
+      return kHint != 0 ? StreamLoad(at) : *at;
+    }
+  };
+  const int key0 = 16 * (qn / 4) + qn % 4;  // this lane's key of key tile 0
+  const uint32_t k_off = ((Q8 ? jg >> 1 : jg) * PT + key0 % PT) * KB + (Q8 ? 16 * (jg & 1) : 0);
+  const uint32_t v_off = qn * PT + 16 * jg % PT;
+  auto load_k = [&](const int (&pg)[PPT], int j) {  // load j = NP kt + p (the four key tiles of a lane lie in one page)
+    kc(j) = read(a.pools.kq + page_head(pg, key0) * (NB * PT * KB), k_off, (j % NP * (Q8 ? 2 : 4) * PT + 4 * (j / NP)) * KB);
+  };
+  auto load_v = [&](const int (&pg)[PPT], int j) {  // q8_0: dim 16 j + qn; q4_0: byte row qn of block j
+    vc(j) = read(a.pools.vq + page_head(pg, 16 * jg) * (Q8 ? D * PT : NB * 16 * PT), v_off, 16 * j * PT);
+  };
+  auto load_scales = [&](const int (&pg)[PPT]) {  // lane: 8 K scales of the tile in [key][block] order, 8 V scales in [block][key]
+    ksr = vsr = uint4{0u, 0u, 0u, 0u};
+    if (lane < NB * 8) {
+      const int key = lane * 8 / NB, chunk = lane % 8;
+      ksr = StreamLoad(reinterpret_cast<const uint4*>(a.pools.ks + (page_head(pg, key) * PT + key % PT) * NB + lane * 8 % NB));
+      vsr = StreamLoad(reinterpret_cast<const uint4*>(a.pools.vs + (page_head(pg, 8 * chunk) * NB + lane / 8) * PT + 8 * chunk % PT));
+    }
+  };
+
+  int pgc[PPT], pgn[PPT];
+  load_pages(tile0, pgn);
+  load_scales(pgn);
+#pragma unroll
+  for (int j = 0; j < NK; ++j) load_k(pgn, j);
+  if constexpr (!kOneSet) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) load_v(pgn, j);
+  }
+  for (int tile = tile0; tile < tile1; tile += step) {
+    // (the last tile's successor is itself: every pass issues the same loads, which keeps the waits exact)
+#pragma unroll
+    for (int j = 0; j < PPT; ++j) pgc[j] = pgn[j];
+    load_pages(tile + step < tile1 ? tile + step : tile, pgn);
+    const bool cut = (tile + 1) * kTile > n_keys;
+    {  // scales to LDS; the V scales of masked keys become 0, which makes their V rows 0 whatever they hold
+      uint32_t w[4] = {vsr.x, vsr.y, vsr.z, vsr.w};
+      if (cut) {
+        const int k0 = tile * kTile + 8 * (lane % 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + e >= n_keys) w[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+      }
+      if (lane < NB * 8) {
+        *reinterpret_cast<uint4*>(&lds.k[lane * 8]) = ksr;
+        *reinterpret_cast<uint4*>(&lds.v[lane * 8]) = uint4{w[0], w[1], w[2], w[3]};
+      }
+      SetSaturation(ksr, uint4{w[0], w[1], w[2], w[3]});
+    }
+    load_scales(pgn);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // ---- S^T
+    f4v st[RB][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      const int key = 16 * (qn / 4) + 4 * kt + qn % 4;
+#pragma unroll
+      for (int i = 0; i < RB; ++i) st[i][kt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const _Float16 d = lds.k[key * NB + (Q8 ? 2 * p + (jg >> 1) : 4 * p + jg)];
+        const h8v d8 = {d, d, d, d, d, d, d, d};
+        const uint4 c = kc(NP * kt + p);
+        h8v ka[SP];
+        if constexpr (Q8) {
+          ka[0] = Codes8(c.x, c.y), ka[1] = Codes8(c.z, c.w);
+        } else {
+          ka[0] = NibblesLo8(c.x, c.y), ka[1] = NibblesLo8(c.z, c.w), ka[2] = NibblesHi8(c.x, c.y), ka[3] = NibblesHi8(c.z, c.w);
+        }
+        if constexpr (kOneSet) load_v(pgc, NP * kt + p);
+        else load_k(pgn, NP * kt + p);
+#pragma unroll
+        for (int sub = 0; sub < SP; ++sub) {
+          ka[sub] *= d8;
+#pragma unroll
+          for (int i = 0; i < RB; ++i)
+            st[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[sub], qb[i][p * SP + sub], st[i][kt], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // ---- numerators: this lane's 16 keys 16 jg + 4 kt + r of its row
+    h8v pv[RB][2];
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      if (cut) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (tile * kTile + 16 * jg + 4 * kt + r >= n_keys) st[i][kt][r] = kNegMax;
+      }
+      float mx = fmaxf(st[i][0][0], st[i][0][1]);
+      mx = fmaxf(fmaxf(mx, st[i][0][2]), st[i][0][3]);
+#pragma unroll
+      for (int kt = 1; kt < 4; ++kt) mx = fmaxf(fmaxf(mx, st[i][kt][0]), st[i][kt][1]), mx = fmaxf(fmaxf(mx, st[i][kt][2]), st[i][kt][3]);
+      mx = OverLaneGroups(mx, [](float x, float y) { return fmaxf(x, y); }) * sscale;
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m[i] + (kBias + kSlack)) != 0, 0)) {
+        const float mn = mx > m[i] + (kBias + kSlack) ? __builtin_ceilf(mx) - kBias : m[i];
+        const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
+        m[i] = mn, l[i] *= alpha;
+        // (the rescaled accumulators go back through a matrix instruction with zero factors: that keeps them in the
+        // accumulation registers on this path as on the common one)
+        const h8v zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          f4v x = o[i][dt];
+          asm volatile("" : "+a"(x));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] *= alpha;
+          o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zero, zero, x, 0, 0, 0);
+        }
+      }
+      const h2v one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+      uint32_t w[2][4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][kt][r], sscale, -m[i]));
+        const h2v p0 = {static_cast<_Float16>(p[0]), static_cast<_Float16>(p[1])};
+        const h2v p1 = {static_cast<_Float16>(p[2]), static_cast<_Float16>(p[3])};
+        // (the sum is of the rounded numerators, as the second product's is)
+        l[i] = __builtin_amdgcn_fdot2(p0, one, l[i], false), l[i] = __builtin_amdgcn_fdot2(p1, one, l[i], false);
+        w[kt / 2][2 * (kt % 2)] = __builtin_bit_cast(uint32_t, p0), w[kt / 2][2 * (kt % 2) + 1] = __builtin_bit_cast(uint32_t, p1);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) pv[i][s] = __builtin_bit_cast(h8v, uint4{w[s][0], w[s][1], w[s][2], w[s][3]});
+    }
+    // ---- O^T
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const h8v s0 = *reinterpret_cast<const h8v*>(&lds.v[b * kTile + 16 * jg]);
+      const h8v s1 = *reinterpret_cast<const h8v*>(&lds.v[b * kTile + 16 * jg + 8]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // dims 32 b + 16 e + 0..15
+        const int dt = 2 * b + e;
+        const uint4 c = vc(Q8 ? dt : b);
+        h8v v0, v1;
+        if constexpr (Q8) v0 = Codes8(c.x, c.y), v1 = Codes8(c.z, c.w);
+        else if (e == 0) v0 = NibblesLo8(c.x, c.y), v1 = NibblesLo8(c.z, c.w);
+        else v0 = NibblesHi8(c.x, c.y), v1 = NibblesHi8(c.z, c.w);
+        if constexpr (Q8) {
+          if constexpr (kOneSet) load_k(pgn, dt);
+          else load_v(pgn, dt);
+        } else if (e == 1) {
+          if constexpr (kOneSet) load_k(pgn, b);
+          else load_v(pgn, b);
+        }
+        v0 *= s0, v1 *= s1;
+#pragma unroll
+        for (int i = 0; i < RB; ++i) o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pv[i][0], o[i][dt], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pv[i][1], o[i][dt], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // (the scales in LDS are rewritten for the next tile)
   }
 }
-// Products beyond the f16 range saturate (they would be infinite, and an infinite score a NaN): only a scale above
-// 65504 / 128 can make one, so the test is one per scale and the slow form is rare.
-constexpr float kLargeScale = 511.0f;
-__device__ __forceinline__ h8v TimesSaturated(h8v codes, h8v scale) {
-  h8v r;
+
+constexpr int kRoundDims = 128;  // dims of a row that the waves' shares meet in LDS with at a time
+template <int D, int RB>
+struct SharedLds {
+  static constexpr int ROWS = 16 * RB, STR = kRoundDims + 4;
+  WaveScales<D> scales[kSharedWaves];
+  float m[kSharedWaves][ROWS], l[kSharedWaves][ROWS];
+  float sums[kSharedWaves][ROWS][STR];
+};
+
+// The four waves' shares of the same rows become one partial in slot `slot` of every live row.
+template <int D, int RB, typename RowOf>
+__device__ __forceinline__ void MergeWaves(const SharedArgs& a, SharedLds<D, RB>& lds, const float (&m)[RB], float (&l)[RB],
+                                           f4v (&o)[RB][D / 16], int n_rows, RowOf row_of, int slot) {
+  constexpr int ROWS = 16 * RB;
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, qn = lane % 16, jg = lane / 16;
+  const int slots = a.n_split + a.tail_split;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = SaturateToF16(static_cast<float>(codes[e]) * static_cast<float>(scale[e]));
-  return r;
+  for (int i = 0; i < RB; ++i) {
+    l[i] = OverLaneGroups(l[i], [](float x, float y) { return x + y; });
+    if (jg == 0) lds.m[wave][16 * i + qn] = m[i], lds.l[wave][16 * i + qn] = l[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    float M = kNone;
+#pragma unroll
+    for (int w = 0; w < kSharedWaves; ++w) M = fmaxf(M, lds.m[w][16 * i + qn]);
+    const float f = __builtin_amdgcn_exp2f(m[i] - M);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[i][dt][r] *= f;
+  }
+  if (tid < ROWS && tid < n_rows) {
+    float M = kNone, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSharedWaves; ++w) M = fmaxf(M, lds.m[w][tid]);
+#pragma unroll
+    for (int w = 0; w < kSharedWaves; ++w) L = __builtin_fmaf(lds.l[w][tid], __builtin_amdgcn_exp2f(lds.m[w][tid] - M), L);
+    *reinterpret_cast<float2*>(&a.ml[(row_of(tid) * slots + slot) * 2]) = float2{M, L};
+  }
+#pragma unroll
+  for (int c = 0; c < D / kRoundDims; ++c) {
+    if (c > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int e = 0; e < kRoundDims / 16; ++e) {
+        const f4v x = o[i][c * (kRoundDims / 16) + e];
+        *reinterpret_cast<float4*>(&lds.sums[wave][16 * i + qn][16 * e + 4 * jg]) = float4{x[0], x[1], x[2], x[3]};
+      }
+    __syncthreads();
+    for (int u = tid; u < min(ROWS, n_rows) * (kRoundDims / 4); u += 64 * kSharedWaves) {
+      const int r = u / (kRoundDims / 4), d = u % (kRoundDims / 4) * 4;
+      float4 v = *reinterpret_cast<const float4*>(&lds.sums[0][r][d]);
+#pragma unroll
+      for (int w = 1; w < kSharedWaves; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(&lds.sums[w][r][d]);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      *reinterpret_cast<float4*>(&a.acc[(row_of(r) * slots + slot) * D + c * kRoundDims + d]) = v;
+    }
+  }
 }
 
-template <int FMT, int D, int PT, int RB, int WR>
+template <int FMT, int D, int PT, int RB>
 __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs a) {
-  constexpr int NB = D / 32, NDT = D / 16, KS = D / 32;
-  constexpr int WK = kSharedWaves / WR, KT = 4 / WK, S2 = 2 / WK;  // 16-key tiles and 32-key steps of a wave
-  static_assert(WK == 1 || WK == 2, "a wave takes whole 32-key steps");
-  constexpr int ROWS = 16 * RB * WR;
-  constexpr int KSTR = D + 8, VSTR = kTile + 8;  // LDS row strides (f16), padded against bank conflicts
-  constexpr int NCH = kTile * D / 16 / 256;      // 16-code chunks of a tile per thread
+  constexpr int ROWS = 16 * RB;
   const Geom g = a.g;
   const int G = g.group(), H = g.n_kv;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
-  const int wr = wave % WR, wk = wave / WR;
-  const int qn = lane % 16, jg = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, qn = lane % 16;
+  __shared__ __align__(16) SharedLds<D, RB> lds;
 
-  // ---- where the tails begin, for the decode kernel behind this one
-  for (int64_t i = int64_t(blockIdx.x) * 256 + tid; i < int64_t(a.n_seqs) * a.tail_stride; i += int64_t(gridDim.x) * 256) {
-    const int s = int(i / a.tail_stride), p = int(i % a.tail_stride), j = GroupOf(a, s);
-    const int len = min(max(a.seq_len[s], 0), a.stride * PT), from = PrefixOf(a, j, len);
-    a.tail_table[i] = a.table[int64_t(s) * a.stride + min(from / PT + p, a.stride - 1)];
-    if (p == 0) a.tail_len[s] = min(len - from, a.max_tail);
+  if (static_cast<int>(blockIdx.x) >= a.prefix_groups) {  // ---- a piece of a tail: the query heads of one kv head of a sequence
+    const int u = blockIdx.x - a.prefix_groups, h = u % H, piece = u / H % a.tail_split, s = u / H / a.tail_split;
+    const Keys k = KeysOf(a, s);
+    const int tiles = (k.tail + kTile - 1) / kTile, per = PerPiece(tiles, a.tail_split);
+    const int tile0 = piece * per, tile1 = min(tile0 + per, tiles);
+    if (tile0 >= tile1) return;
+    const size_t row0 = size_t(s) * g.n_q + size_t(h) * G;
+    const size_t prow[1] = {row0 + min(qn, G - 1)};
+    float m[1], l[1];
+    f4v o[1][D / 16];
+    StreamKeys<FMT, D, PT, 1>(a, a.table + int64_t(s) * a.stride, k.prefix, h, tile0 + wave, kSharedWaves, tile1, k.tail, prow,
+                              lds.scales[wave], m, l, o);
+    MergeWaves<D, 1>(a, reinterpret_cast<SharedLds<D, 1>&>(lds), m, l, o, G, [&](int r) { return row0 + r; }, a.n_split + piece);
+    return;
   }
-
-  // ---- this workgroup's rows and keys. Workgroups that read the same keys (the row blocks of a piece of a prefix) run on
-  // one XCD, side by side.
+  // ---- a piece of a prefix against a block of its group's rows. Workgroups that read the same keys (the row blocks of a
+  // piece) run on one XCD, side by side.
   const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
   const int pair = xcd + 8 * (local / a.max_blocks), block = local % a.max_blocks;
   if (pair >= H * a.n_split) return;
@@ -135,8 +454,8 @@ __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs
     }
     const unsigned long long mine = __ballot(before + incl > block && before + incl - n <= block);
     if (mine != 0) {
-      const int l = __builtin_ctzll(mine);
-      group = j0 + l, row0 = (block - before - __shfl(incl - n, l, 64)) * ROWS;
+      const int at = __builtin_ctzll(mine);
+      group = j0 + at, row0 = (block - before - __shfl(incl - n, at, 64)) * ROWS;
       break;
     }
     before += __shfl(incl, 63, 64);
@@ -144,258 +463,48 @@ __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs
   group = __builtin_amdgcn_readfirstlane(group), row0 = __builtin_amdgcn_readfirstlane(row0);
   if (group < 0) return;
   const int first = GroupFirst(a, group), n_rows = (GroupFirst(a, group + 1) - first) * G;
-  const int shared = GroupShared(a, group), tiles = shared / kTile;
-  const int per = TilesPerPiece(tiles, a.n_split);
+  const int shared = GroupShared(a, group), tiles = shared / kTile, per = PerPiece(tiles, a.n_split);
   const int tile0 = piece * per, tile1 = min(tile0 + per, tiles);
   if (tile0 >= tile1) return;
-
-  __shared__ __align__(16) _Float16 lk[kTile][KSTR];  // K tile, [key][dim]
-  __shared__ __align__(16) _Float16 lv[D][VSTR];      // V^T tile, [dim][key]
-  __shared__ __align__(16) _Float16 lvs[NB][kTile];   // V scales of the tile, [block][key]
-  __shared__ int large_v;                             // some of them are above kLargeScale
-
-  h8v qb[RB][KS];
-  size_t prow[RB];  // (sequence, query head) of this lane's row in block i
-  bool live[RB];    // it exists and its sequence is as long as the prefix
-#pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    const int r = row0 + (wr * RB + i) * 16 + qn, rr = min(r, n_rows - 1);
-    const int s = first + rr / G;
-    live[i] = r < n_rows && min(a.seq_len[s], a.stride * PT) >= shared;
-    prow[i] = size_t(s) * g.n_q + size_t(h) * G + rr % G;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qb[i][ks] = LoadQ8(a.q, prow[i] * D + 32 * ks + 8 * jg, a.q_dtype);
-  }
-  f4v o[RB][NDT], lacc[RB];
-  float m[RB];
-#pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    m[i] = kNone, lacc[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[i][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  const float sscale = a.scale * 1.4426950408889634f;
-  const int32_t* row = a.table + int64_t(first) * a.stride;
-  auto page_head = [&](int key) -> size_t { return size_t(ClampPage(row[key / PT], g.n_pages)) * H + h; };
-
-  uint4 kraw[NCH], vraw[NCH], vsr;
-  uint16_t ksr[NCH];
-  auto fetch_k = [&](int tile) {  // chunk c: block c / 128, key (c % 128) / 2, half c % 2
-#pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int c = tid + 256 * j, b = c / 128, key = (c % 128) / 2, hf = c % 2, kk = tile * kTile + key;
-      const size_t ph = page_head(kk);
-      kraw[j] = FMT == 8 ? *reinterpret_cast<const uint4*>(a.pools.kq + ((ph * NB + b) * PT + kk % PT) * 32 + 16 * hf)
-                         : *reinterpret_cast<const uint4*>(a.pools.kq + ((ph * NB + b) * PT + kk % PT) * 16);
-      ksr[j] = a.pools.ks[(ph * PT + kk % PT) * NB + b];
-    }
+  auto row_of = [&](int r) -> size_t {  // row r of the block: its place among all (sequence, query head) rows
+    const int rr = min(row0 + r, n_rows - 1);
+    return (size_t(first) + rr / G) * g.n_q + size_t(h) * G + rr % G;
   };
-  auto stage_k = [&](int j) {
-    const int c = tid + 256 * j, b = c / 128, key = (c % 128) / 2, hf = c % 2;
-    const _Float16 d = __builtin_bit_cast(_Float16, ksr[j]);
-    const h8v d8 = {d, d, d, d, d, d, d, d};
-    h8v lo, hi;
-    Halves<FMT>(kraw[j], hf, &lo, &hi);
-    if (__builtin_expect(__ballot(!(fabsf(static_cast<float>(d)) <= kLargeScale)) != 0, 0))
-      lo = TimesSaturated(lo, d8), hi = TimesSaturated(hi, d8);
-    else
-      lo *= d8, hi *= d8;
-    h8v* dst = reinterpret_cast<h8v*>(&lk[key][32 * b + 16 * hf]);
-    dst[0] = lo, dst[1] = hi;
-  };
-  auto fetch_v = [&](int tile) {  // chunk c: dim c / 4, keys 16 (c % 4) .. + 15
+  size_t prow[RB];
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int c = tid + 256 * j, d = c / 4, kk = tile * kTile + 16 * (c % 4);
-      const size_t ph = page_head(kk);
-      vraw[j] = FMT == 8 ? *reinterpret_cast<const uint4*>(a.pools.vq + (ph * D + d) * PT + kk % PT)
-                         : *reinterpret_cast<const uint4*>(a.pools.vq + ((ph * NB + d / 32) * 16 + d % 16) * PT + kk % PT);
-    }
-  };
-  auto fetch_vs = [&](int tile) {  // thread = (block, 8 keys)
-    if (tid < NB * 8) {
-      const int b = tid / 8, kk = tile * kTile + 8 * (tid % 8);
-      vsr = *reinterpret_cast<const uint4*>(a.pools.vs + (page_head(kk) * NB + b) * PT + kk % PT);
-    }
-  };
-  auto stage_vs = [&]() {
-    if (tid < 64) {  // (NB * 8 threads: one wave, or half of one)
-      bool large = false;
-      if (tid < NB * 8) {
-        const h8v sc = __builtin_bit_cast(h8v, vsr);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) large |= !(fabsf(static_cast<float>(sc[e])) <= kLargeScale);
-        *reinterpret_cast<uint4*>(&lvs[tid / 8][8 * (tid % 8)]) = vsr;
-      }
-      const bool any = __ballot(large) != 0;
-      if (tid == 0) large_v = any;
-    }
-  };
-  auto stage_v = [&](int j) {
-    const int c = tid + 256 * j, d = c / 4, k0 = 16 * (c % 4);
-    const h8v s0 = *reinterpret_cast<const h8v*>(&lvs[d / 32][k0]), s1 = *reinterpret_cast<const h8v*>(&lvs[d / 32][k0 + 8]);
-    h8v lo, hi;
-    Halves<FMT>(vraw[j], d % 32 / 16, &lo, &hi);
-    if (__builtin_expect(large_v != 0, 0)) lo = TimesSaturated(lo, s0), hi = TimesSaturated(hi, s1);
-    else lo *= s0, hi *= s1;
-    h8v* dst = reinterpret_cast<h8v*>(&lv[d][k0]);
-    dst[0] = lo, dst[1] = hi;
-  };
-
-  // Pipeline: while the matrix cores run a tile's K Q^T out of lk, the vector units decode its V into lv; while they run
-  // V^T P^T out of lv, the next tile's K is decoded into lk. Codes are fetched a tile before they are decoded.
-  fetch_k(tile0);
-  fetch_vs(tile0);
-  fetch_v(tile0);
-#pragma unroll
-  for (int j = 0; j < NCH; ++j) stage_k(j);
-  stage_vs();
-  if (tile0 + 1 < tile1) fetch_k(tile0 + 1), fetch_vs(tile0 + 1);
-  __syncthreads();
-  for (int tile = tile0; tile < tile1; ++tile) {
-    f4v st[RB][KT];
-#pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) st[i][kt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      h8v ka[KT];
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) ka[kt] = *reinterpret_cast<const h8v*>(&lk[16 * (wk * KT + kt) + qn][32 * ks + 8 * jg]);
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int i = 0; i < RB; ++i) st[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kt], qb[i][ks], st[i][kt], 0, 0, 0);
-      if (ks % (KS / NCH) == KS / NCH - 1) stage_v(ks / (KS / NCH));
-    }
-    if (tile + 1 < tile1) fetch_v(tile + 1);
-    h8v pv[RB][S2];
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      float mx = kNegMax;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = st[i][kt][r] * sscale;
-          st[i][kt][r] = v;
-          mx = fmaxf(mx, v);
-        }
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m[i], __builtin_ceilf(mx) - kBias);  // whole numbers: rescaling is exact
-      const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
-      m[i] = mn;
-      uint32_t w[S2][4];
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        _Float16 p[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = static_cast<_Float16>(__builtin_amdgcn_exp2f(st[i][kt][r] - mn));
-        // 32-key step kt / 2 takes keys 4 jg + r of its even 16-key tile, then of its odd one
-        w[kt / 2][2 * (kt % 2)] = __builtin_bit_cast(uint32_t, h2v{p[0], p[1]});
-        w[kt / 2][2 * (kt % 2) + 1] = __builtin_bit_cast(uint32_t, h2v{p[2], p[3]});
-      }
-#pragma unroll
-      for (int s2 = 0; s2 < S2; ++s2) pv[i][s2] = __builtin_bit_cast(h8v, uint4{w[s2][0], w[s2][1], w[s2][2], w[s2][3]});
-      if (__ballot(alpha != 1.0f) != 0) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) lacc[i][r] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[i][dt][r] *= alpha;
-      }
-    }
-    __syncthreads();  // every wave is done with lk, and the tile's V is complete in lv
-    const h8v ones = __builtin_bit_cast(h8v, uint4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
-#pragma unroll
-    for (int s2 = 0; s2 < S2; ++s2)
-#pragma unroll
-      for (int i = 0; i < RB; ++i) lacc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pv[i][s2], lacc[i], 0, 0, 0);
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-#pragma unroll
-      for (int s2 = 0; s2 < S2; ++s2) {
-        const uint2 v0 = *reinterpret_cast<const uint2*>(&lv[16 * dt + qn][32 * (wk * S2 + s2) + 4 * jg]);
-        const uint2 v1 = *reinterpret_cast<const uint2*>(&lv[16 * dt + qn][32 * (wk * S2 + s2) + 16 + 4 * jg]);
-        const h8v va = __builtin_bit_cast(h8v, uint4{v0.x, v0.y, v1.x, v1.y});
-#pragma unroll
-        for (int i = 0; i < RB; ++i) o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pv[i][s2], o[i][dt], 0, 0, 0);
-      }
-      if (tile + 1 < tile1 && dt % (NDT / NCH) == NDT / NCH - 1) stage_k(dt / (NDT / NCH));
-    }
-    stage_vs();  // (of the next tile, or once more the last one's)
-    if (tile + 2 < tile1) fetch_k(tile + 2), fetch_vs(tile + 2);
-    __syncthreads();  // every wave is done with lv; the next tile's K and V scales are in place
-  }
-#pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    if (!live[i]) continue;
-    const size_t at = prow[i] * a.slots + piece * WK + wk;
-    if (jg == 0) *reinterpret_cast<float2*>(&a.ml[at * 2]) = float2{m[i], lacc[i][0]};
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
-      *reinterpret_cast<float4*>(&a.acc[at * D + 16 * dt + 4 * jg]) = float4{o[i][dt][0], o[i][dt][1], o[i][dt][2], o[i][dt][3]};
-  }
+  for (int i = 0; i < RB; ++i) prow[i] = row_of(16 * i + qn);
+  float m[RB], l[RB];
+  f4v o[RB][D / 16];
+  StreamKeys<FMT, D, PT, RB>(a, a.table + int64_t(first) * a.stride, 0, h, tile0 + wave, kSharedWaves, tile1, shared, prow,
+                             lds.scales[wave], m, l, o);
+  // (rows of sequences shorter than the prefix leave partials that nobody reads)
+  MergeWaves<D, RB>(a, lds, m, l, o, n_rows - row0, row_of, piece);
 }
 
 // One workgroup per (query head, sequence): the prefix's partials and the tail's, weighed by 2^(m - M) and 1 / l. A group of
 // D / 4 lanes takes every n-th partial, four dims a lane; the groups' sums meet in LDS.
 struct MergeArgs {
   SharedArgs s;
-  DecodeArgs tail;
-  int32_t waves_along_keys;
   const float* gate;
   void* out;
   int32_t out_dtype;
 };
 constexpr int kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void SharedMerge(const MergeArgs a) {
-  constexpr float kLog2e = 1.4426950408889634f;
   const Geom g = a.s.g;
-  const int D = g.hd, G = g.group(), H = g.n_kv, hq = blockIdx.x, s = blockIdx.y, t = threadIdx.x, h = hq / G, gi = hq % G;
+  const int D = g.hd, hq = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
   const size_t row = size_t(s) * g.n_q + hq;
-  // the prefix's pieces
-  const int j = GroupOf(a.s, s);
-  const int tiles = PrefixOf(a.s, j, min(max(a.s.seq_len[s], 0), a.s.stride * g.pt)) / kTile;
-  const int per = max(TilesPerPiece(tiles, a.s.n_split), 1);
-  const int n_pre = (tiles + per - 1) / per * a.waves_along_keys;
-  // the places of the tail's partials (decode_cut.hpp)
-  const DecodeArgs& d = a.tail;
-  const int ts = TilesOf(d, s);
-  size_t p0 = 0, p1 = 0;
-  if (ts > 0) {
-    const int Hc = CutHeads(d);
-    const long long A = ChunkUnits(d, static_cast<long long>(d.tprefix[d.n_seqs]) * Hc);
-    const long long first = static_cast<long long>(d.tprefix[s]) * Hc +
-                            static_cast<long long>(Hc == 1 ? 0 : h) * UnitsOf(d, ts) + d.pair_cost;
-    const int k0 = ChunkOf(d, A, first), k1 = ChunkOf(d, A, first + ts - 1);
-    p0 = size_t(k0 + s * H + h) * d.wpc, p1 = size_t(k1 + s * H + h + 1) * d.wpc;
-    if (Hc == 1 && H > 1) {
-      const size_t r = size_t(h) * (d.n_chunks + d.n_seqs) + s;
-      p0 = (r + k0) * d.wpc, p1 = (r + k1 + 1) * d.wpc;
-    }
-  }
-  const int n = n_pre + static_cast<int>(p1 - p0);
-  // partial i: reference point in base 2 and sum (0: nothing there, and its accumulator was not written)
-  auto ml_of = [&](int i) -> float2 {
-    if (i < n_pre) return *reinterpret_cast<const float2*>(&a.s.ml[(row * a.s.slots + i) * 2]);
-    const float2 v = *reinterpret_cast<const float2*>(&d.ml[((p0 + (i - n_pre)) * G + gi) * 2]);
-    return float2{v.x * kLog2e, v.y};
-  };
-  auto acc_of = [&](int i) -> const float* {
-    return i < n_pre ? &a.s.acc[(row * a.s.slots + i) * D] : &d.acc[((p0 + (i - n_pre)) * G + gi) * D];
-  };
+  const int slots = a.s.n_split + a.s.tail_split;
+  const Keys k = KeysOf(a.s, s);
+  const int pre_tiles = k.prefix / kTile, tail_tiles = (k.tail + kTile - 1) / kTile;
+  const int pre_per = PerPiece(pre_tiles, a.s.n_split), tail_per = PerPiece(tail_tiles, a.s.tail_split);
+  const int n_pre = (pre_tiles + pre_per - 1) / pre_per, n = n_pre + (tail_tiles + tail_per - 1) / tail_per;
+  auto slot_of = [&](int i) -> size_t { return row * slots + (i < n_pre ? i : a.s.n_split + i - n_pre); };
   __shared__ float red[kMergeThreads / 64];
   __shared__ __align__(16) float sums[kMergeThreads * 4];
   __shared__ float lsum[kMergeThreads / 32];
   float M = kNegMax;
-  for (int i = t; i < n; i += kMergeThreads) {
-    const float2 v = ml_of(i);
-    if (v.y > 0.0f) M = fmaxf(M, v.x);
-  }
+  for (int i = t; i < n; i += kMergeThreads) M = fmaxf(M, a.s.ml[slot_of(i) * 2]);
   M = WaveMax(M);
   if (t % 64 == 0) red[t / 64] = M;
   __syncthreads();
@@ -404,14 +513,12 @@ __global__ __launch_bounds__(kMergeThreads) void SharedMerge(const MergeArgs a) 
   const int lanes = D / 4, grp = t / lanes, dl = t % lanes, groups = kMergeThreads / lanes;
   float4 A = {0.0f, 0.0f, 0.0f, 0.0f};
   float L = 0.0f;
+#pragma unroll 4
   for (int i = grp; i < n; i += groups) {
-    const float2 v = ml_of(i);
-    if (!(v.y > 0.0f)) {
-      if (v.y != v.y) L = v.y;  // NaN queries or pools: the row is NaN, as in the decode attention
-      continue;
-    }
+    const size_t at = slot_of(i);
+    const float2 v = *reinterpret_cast<const float2*>(&a.s.ml[at * 2]);
+    const float4 x = *reinterpret_cast<const float4*>(&a.s.acc[at * D + 4 * dl]);
     const float w = __builtin_amdgcn_exp2f(v.x - M);
-    const float4 x = *reinterpret_cast<const float4*>(acc_of(i) + 4 * dl);
     A.x = __builtin_fmaf(w, x.x, A.x), A.y = __builtin_fmaf(w, x.y, A.y);
     A.z = __builtin_fmaf(w, x.z, A.z), A.w = __builtin_fmaf(w, x.w, A.w);
     L = __builtin_fmaf(w, v.y, L);
@@ -420,60 +527,62 @@ __global__ __launch_bounds__(kMergeThreads) void SharedMerge(const MergeArgs a) 
   if (dl == 0) lsum[grp] = L;
   __syncthreads();
   for (int e = t; e < D; e += kMergeThreads) {
-    float v = 0.0f, l = 0.0f;
-    for (int q = 0; q < groups; ++q) v += sums[q * D + e], l += lsum[q];
-    v = l == 0.0f ? 0.0f : v / l;  // (a sequence without keys)
+    float v = 0.0f, sum = 0.0f;
+    for (int q = 0; q < groups; ++q) v += sums[q * D + e], sum += lsum[q];
+    v = n == 0 ? 0.0f : v / sum;  // (a sequence without keys)
     if (a.gate != nullptr) v *= 1.0f / (1.0f + __expf(-a.gate[row * D + e]));
     Store1(a.out, row * D + e, a.out_dtype, v);
   }
 }
 
 struct SharedPlan {
-  int rows, waves_along_keys;  // query rows of a workgroup
-  int32_t max_blocks, n_split, slots, tail_stride;
-  size_t off_len, off_table, off_ml, off_acc, off_part, part_bytes, bytes;
+  int row_blocks;  // of 16 query rows, that a wave of a prefix takes
+  int32_t max_blocks, n_split, tail_split, prefix_groups;
+  int64_t groups;  // workgroups in all
+  size_t off_ml, off_acc, bytes;
 };
 SharedPlan MakeSharedPlan(const Geom& m, int32_t n_seqs, int32_t n_groups, int32_t max_shared, int32_t max_tail) {
   SharedPlan p;
-  const int64_t rows = int64_t(n_seqs) * m.group();
-  // A workgroup's rows follow the rows of an average group: fewer, and the tile's decode is paid more often; more, and
-  // matrix rows go unused.
-  const int64_t per_group = (rows + n_groups - 1) / n_groups;
-  p.rows = per_group <= 32 ? 32 : per_group <= 64 ? 64 : 128;
-  p.waves_along_keys = p.rows == 128 ? 1 : 2;
-  p.max_blocks = static_cast<int32_t>(rows / p.rows + n_groups);
-  const int64_t max_tiles = max_shared / kTile;
-  const int64_t want = (2 * int64_t(ComputeUnits()) + int64_t(p.max_blocks) * m.n_kv - 1) / (int64_t(p.max_blocks) * m.n_kv);
-  p.n_split = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(want, (max_tiles + 3) / 4)));
-  p.slots = max_tiles > 0 ? p.n_split * p.waves_along_keys : 0;
-  p.tail_stride = (max_tail + m.pt - 1) / m.pt;
-  const size_t parts = size_t(n_seqs) * m.n_q * p.slots;
-  p.off_len = 0;
-  p.off_table = Align(sizeof(int32_t) * size_t(n_seqs));
-  p.off_ml = Align(p.off_table + sizeof(int32_t) * size_t(n_seqs) * p.tail_stride);
-  p.off_acc = Align(p.off_ml + sizeof(float) * 2 * parts);
-  p.off_part = Align(p.off_acc + sizeof(float) * parts * m.hd);
-  p.part_bytes = MakePlan(m, n_seqs, max_tail, MakeTuning(nullptr)).bytes;
-  p.bytes = p.off_part + p.part_bytes;
+  const int64_t rows = int64_t(n_seqs) * m.group(), per_group = (rows + n_groups - 1) / n_groups;
+  auto blocks = [&](int rb) { return (per_group + 16 * rb - 1) / (16 * rb); };
+  // A tile costs a wave about 4000 cycles of decoding and 1500 for each block of 16 rows, whether or not the rows exist.
+  p.row_blocks = 1;
+  for (int rb = 2; rb <= 3; ++rb)
+    if (blocks(rb) * (8 + 3 * rb) < blocks(p.row_blocks) * (8 + 3 * p.row_blocks)) p.row_blocks = rb;
+  p.max_blocks = static_cast<int32_t>(n_groups == 1 ? blocks(p.row_blocks) : rows / (16 * p.row_blocks) + n_groups);
+  // One workgroup per CU and round. A prefix is cut so that the row blocks of an average group fill one round, a tail into
+  // pieces of at most sixteen tiles (four a wave), and finer while that leaves CUs idle; a piece has a tile for every wave.
+  const int64_t cus = ComputeUnits(), pre_tiles = max_shared / kTile, tail_tiles = (int64_t(max_tail) + kTile - 1) / kTile;
+  const int64_t per_piece = std::max<int64_t>(1, std::min<int64_t>(int64_t(n_groups) * blocks(p.row_blocks), p.max_blocks)) * m.n_kv;
+  p.n_split = static_cast<int32_t>(std::max<int64_t>(1, std::min((cus + per_piece / 2) / per_piece, (pre_tiles + 3) / 4)));
+  if (pre_tiles == 0) p.n_split = 0;
+  const int64_t tails = int64_t(n_seqs) * m.n_kv;
+  p.tail_split = static_cast<int32_t>(std::max<int64_t>(1, std::min(std::max((cus + tails - 1) / tails, (tail_tiles + 15) / 16), (tail_tiles + 3) / 4)));
+  p.prefix_groups = static_cast<int32_t>((int64_t(m.n_kv) * p.n_split + 7) / 8 * 8 * p.max_blocks);
+  p.groups = p.prefix_groups + tails * p.tail_split;
+  const size_t parts = size_t(n_seqs) * m.n_q * (p.n_split + p.tail_split);
+  p.off_ml = 0;
+  p.off_acc = Align(sizeof(float) * 2 * parts);
+  p.bytes = Align(p.off_acc + sizeof(float) * parts * m.hd);
   return p;
 }
 
 template <int FMT, int D, int PT>
-void LaunchShared(const SharedArgs& a, int rows, dim3 grid, hipStream_t st) {
+void LaunchShared(const SharedArgs& a, int row_blocks, dim3 grid, hipStream_t st) {
   const dim3 block(64 * kSharedWaves);
-  if (rows == 128) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 2, 4>), grid, block, 0, st, a);
-  else if (rows == 64) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 2, 2>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((SharedPart<FMT, D, PT, 1, 2>), grid, block, 0, st, a);
+  if (row_blocks == 3) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 3>), grid, block, 0, st, a);
+  else if (row_blocks == 2) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 2>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((SharedPart<FMT, D, PT, 1>), grid, block, 0, st, a);
 }
 template <int FMT>
-void LaunchSharedFormat(const SharedArgs& a, int rows, dim3 grid, hipStream_t st) {
+void LaunchSharedFormat(const SharedArgs& a, int row_blocks, dim3 grid, hipStream_t st) {
   const Geom& m = a.g;
-  if (m.hd == 256 && m.pt == 64) LaunchShared<FMT, 256, 64>(a, rows, grid, st);
-  else if (m.hd == 256 && m.pt == 32) LaunchShared<FMT, 256, 32>(a, rows, grid, st);
-  else if (m.hd == 256) LaunchShared<FMT, 256, 16>(a, rows, grid, st);
-  else if (m.pt == 64) LaunchShared<FMT, 128, 64>(a, rows, grid, st);
-  else if (m.pt == 32) LaunchShared<FMT, 128, 32>(a, rows, grid, st);
-  else LaunchShared<FMT, 128, 16>(a, rows, grid, st);
+  if (m.hd == 256 && m.pt == 64) LaunchShared<FMT, 256, 64>(a, row_blocks, grid, st);
+  else if (m.hd == 256 && m.pt == 32) LaunchShared<FMT, 256, 32>(a, row_blocks, grid, st);
+  else if (m.hd == 256) LaunchShared<FMT, 256, 16>(a, row_blocks, grid, st);
+  else if (m.pt == 64) LaunchShared<FMT, 128, 64>(a, row_blocks, grid, st);
+  else if (m.pt == 32) LaunchShared<FMT, 128, 32>(a, row_blocks, grid, st);
+  else LaunchShared<FMT, 128, 16>(a, row_blocks, grid, st);
 }
 
 int CheckSharedShape(const yahkv_geometry* g, int32_t n_seqs, int32_t n_groups, int32_t max_shared_len, int32_t max_tail_len) {
@@ -510,30 +619,23 @@ extern "C" int yahkv_decode_attend_shared(const yahkv_geometry* g, const yahkv_p
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return YAHKV_ERR_ARG;
   const Geom m = MakeGeom(*g);
-  if (int64_t(page_table_stride) * m.pt > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
+  if (int64_t(page_table_stride) * m.pt > 0x7FFFFFFF - kTile * kSharedWaves) return YAHKV_ERR_SHAPE;
   const SharedPlan p = MakeSharedPlan(m, n_seqs, n_groups, max_shared_len, max_tail_len);
   if (workspace_bytes < p.bytes) return YAHKV_ERR_WORKSPACE;
-  const int64_t blocks = (int64_t(m.n_kv) * p.n_split + 7) / 8 * 8 * p.max_blocks;
-  if (blocks > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
+  if (p.groups > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
   char* ws = static_cast<char*>(workspace);
   SharedArgs a{};
   a.g = m, a.pools = MakePools(*pools), a.table = page_table, a.seq_len = seq_len, a.group_first = group_first;
   a.shared_len = shared_len, a.stride = page_table_stride, a.n_seqs = n_seqs, a.n_groups = n_groups;
   a.max_shared = max_shared_len, a.max_tail = max_tail_len, a.q = q, a.q_dtype = q_dtype, a.scale = softmax_scale;
-  a.max_blocks = p.max_blocks, a.n_split = p.n_split, a.slots = p.slots, a.tail_stride = p.tail_stride;
-  a.tail_len = reinterpret_cast<int32_t*>(ws + p.off_len), a.tail_table = reinterpret_cast<int32_t*>(ws + p.off_table);
+  a.max_blocks = p.max_blocks, a.n_split = p.n_split, a.tail_split = p.tail_split, a.prefix_groups = p.prefix_groups;
   a.ml = reinterpret_cast<float*>(ws + p.off_ml), a.acc = reinterpret_cast<float*>(ws + p.off_acc);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  MergeArgs ma{};
-  if (const int rc = Prepare(m, p.tail_stride, a.tail_len, n_seqs, max_tail_len, ws + p.off_part, p.part_bytes, nullptr, &ma.tail)) return rc;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (m.format == YAHKV_Q8_0) LaunchSharedFormat<8>(a, p.rows, grid, st);
-  else LaunchSharedFormat<4>(a, p.rows, grid, st);
+  const dim3 grid(static_cast<unsigned>(p.groups));
+  if (m.format == YAHKV_Q8_0) LaunchSharedFormat<8>(a, p.row_blocks, grid, st);
+  else LaunchSharedFormat<4>(a, p.row_blocks, grid, st);
   if (const int rc = LaunchStatus()) return rc;
-  if (const int rc = yahkv_decode_part(g, pools, a.tail_table, p.tail_stride, a.tail_len, n_seqs, max_tail_len, q, q_dtype,
-                                       softmax_scale, ws + p.off_part, p.part_bytes, nullptr, stream))
-    return rc;
-  ma.s = a, ma.waves_along_keys = p.waves_along_keys, ma.gate = gate, ma.out = out, ma.out_dtype = out_dtype;
+  const MergeArgs ma{a, gate, out, out_dtype};
   hipLaunchKernelGGL(SharedMerge, dim3(static_cast<unsigned>(m.n_q), static_cast<unsigned>(n_seqs)), dim3(kMergeThreads), 0, st, ma);
   return LaunchStatus();
 }
