@@ -118,12 +118,53 @@ struct WaveScales {  // a tile's scales in LDS, [key][block] and [block][key]
   _Float16 k[kTile * D / 32], v[D / 32 * kTile];
 };
 
+// A workgroup's query rows on their way to LDS, as f16: asked for first, converted when the first tile's loads are out too.
+// (Converted by every wave for its own operands, in all three types of the source, they were half of the kernel's code; a
+// workgroup runs most of its code once or a few times, and fetching it was what a small call waited for.)
+template <int D, int RB>
+struct QueryRows {
+  static constexpr int ROWS = 16 * RB, STR = D + 8, PER = ROWS * (D / 8) / (64 * kSharedWaves);
+  _Float16 (*lds)[STR];
+  RawQ8 raw[PER];
+  template <typename RowOf>
+  __device__ __forceinline__ void Request(const void* q, int dtype, RowOf row_of) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int u = threadIdx.x + 64 * kSharedWaves * j;
+      raw[j] = LoadRawQ8(q, row_of(u / (D / 8)) * D + u % (D / 8) * 8, dtype);
+    }
+  }
+  __device__ __forceinline__ void Stage(int dtype) {
+    auto put = [&](int j, h8v v) {
+      const int u = threadIdx.x + 64 * kSharedWaves * j;
+      *reinterpret_cast<h8v*>(&lds[u / (D / 8)][u % (D / 8) * 8]) = v;
+    };
+    if (dtype == YAHKV_F16) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) put(j, __builtin_bit_cast(h8v, raw[j].a));
+    } else if (dtype == YAHKV_BF16) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) put(j, ConvertQ8(raw[j], YAHKV_BF16));
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) put(j, ConvertQ8(raw[j], YAHKV_F32));
+    }
+    // (a bare barrier behind the LDS writes: __syncthreads() would wait for the codes on their way in as well)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  __device__ __forceinline__ h8v At(int row, int d) const { return *reinterpret_cast<const h8v*>(&lds[row][d]); }
+};
+
 // Tiles tile0, tile0 + step, .. below tile1 of the sequence behind table row `row`, from key `origin` on, `n_keys` keys in
-// all (those at or past it are masked), against RB row blocks (query rows prow[]): reference points, this lane's part of the
-// sums, accumulators.
+// all (those at or past it are masked), against RB row blocks: reference points, this lane's part of the sums, accumulators.
+// All four waves of the workgroup call it together (the queries go through LDS behind one barrier); a wave without a tile
+// loads one all the same.
 template <int FMT, int D, int PT, int RB>
 __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* row, int origin, int h, int tile0, int step,
-                                           int tile1, int n_keys, const size_t (&prow)[RB], WaveScales<D>& lds, float (&m)[RB],
+                                           int tile1, int n_keys, QueryRows<D, RB>& queries, WaveScales<D>& lds, float (&m)[RB],
                                            float (&l)[RB], f4v (&o)[RB][D / 16]) {
   constexpr int NB = D / 32, NDT = D / 16, KS = D / 32, PPT = kTile / PT;
   constexpr bool Q8 = FMT == 8;
@@ -132,20 +173,6 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
   constexpr int NV = Q8 ? NDT : NB;         // V loads
   const Geom& g = a.g;
   const int H = g.n_kv, lane = threadIdx.x % 64, qn = lane % 16, jg = lane / 16;
-  // dims of step (p, sub) that this lane group holds
-  auto dims = [&](int p, int sub) -> int {
-    return Q8 ? 32 * (2 * p + (jg >> 1)) + 16 * (jg & 1) + 8 * sub : 32 * (4 * p + jg) + 8 * (sub & 1) + 16 * (sub >> 1);
-  };
-  h8v qb[RB][KS];
-#pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    m[i] = kNone, l[i] = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qb[i][ks] = LoadQ8(a.q, prow[i] * D + dims(ks / SP, ks % SP), a.q_dtype);
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[i][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  if (tile0 >= tile1) return;
   const float sscale = a.scale * 1.4426950408889634f;
 
   // pages of a tile, through the constant address space (scalar loads, which the vector memory counter does not see)
@@ -213,6 +240,21 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
   if constexpr (!kOneSet) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) load_v(pgn, j);
+  }
+  // the queries, which were asked for before all this: through LDS into the first product's operands
+  queries.Stage(a.q_dtype);
+  h8v qb[RB][KS];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    m[i] = kNone, l[i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {  // the dims of step (p, sub) that this lane group holds
+      const int p = ks / SP, sub = ks % SP;
+      qb[i][ks] = queries.At(16 * i + qn, Q8 ? 32 * (2 * p + (jg >> 1)) + 16 * (jg & 1) + 8 * sub
+                                             : 32 * (4 * p + jg) + 8 * (sub & 1) + 16 * (sub >> 1));
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[i][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   }
   for (int tile = tile0; tile < tile1; tile += step) {
     // (the last tile's successor is itself: every pass issues the same loads, which keeps the waits exact)
@@ -354,7 +396,10 @@ struct SharedLds {
   static constexpr int ROWS = 16 * RB, STR = kRoundDims + 4;
   WaveScales<D> scales[kSharedWaves];
   float m[kSharedWaves][ROWS], l[kSharedWaves][ROWS];
-  float sums[kSharedWaves][ROWS][STR];
+  union {
+    _Float16 q[ROWS][D + 8];  // until every wave has its operands
+    float sums[kSharedWaves][ROWS][STR];  // (MergeWaves writes it behind a barrier)
+  };
 };
 
 // The four waves' shares of the same rows become one partial in slot `slot` of every live row.
@@ -418,7 +463,7 @@ __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs
   constexpr int ROWS = 16 * RB;
   const Geom g = a.g;
   const int G = g.group(), H = g.n_kv;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, qn = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   __shared__ __align__(16) SharedLds<D, RB> lds;
 
   if (static_cast<int>(blockIdx.x) >= a.prefix_groups) {  // ---- a piece of a tail: the query heads of one kv head of a sequence
@@ -428,12 +473,15 @@ __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs
     const int tile0 = piece * per, tile1 = min(tile0 + per, tiles);
     if (tile0 >= tile1) return;
     const size_t row0 = size_t(s) * g.n_q + size_t(h) * G;
-    const size_t prow[1] = {row0 + min(qn, G - 1)};
+    auto& lds1 = reinterpret_cast<SharedLds<D, 1>&>(lds);
+    QueryRows<D, 1> queries;
+    queries.lds = lds1.q;
+    queries.Request(a.q, a.q_dtype, [&](int r) { return row0 + min(r, G - 1); });
     float m[1], l[1];
     f4v o[1][D / 16];
-    StreamKeys<FMT, D, PT, 1>(a, a.table + int64_t(s) * a.stride, k.prefix, h, tile0 + wave, kSharedWaves, tile1, k.tail, prow,
-                              lds.scales[wave], m, l, o);
-    MergeWaves<D, 1>(a, reinterpret_cast<SharedLds<D, 1>&>(lds), m, l, o, G, [&](int r) { return row0 + r; }, a.n_split + piece);
+    StreamKeys<FMT, D, PT, 1>(a, a.table + int64_t(s) * a.stride, k.prefix, h, tile0 + wave, kSharedWaves, tile1, k.tail, queries,
+                              lds1.scales[wave], m, l, o);
+    MergeWaves<D, 1>(a, lds1, m, l, o, G, [&](int r) { return row0 + r; }, a.n_split + piece);
     return;
   }
   // ---- a piece of a prefix against a block of its group's rows. Workgroups that read the same keys (the row blocks of a
@@ -470,12 +518,12 @@ __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs
     const int rr = min(row0 + r, n_rows - 1);
     return (size_t(first) + rr / G) * g.n_q + size_t(h) * G + rr % G;
   };
-  size_t prow[RB];
-#pragma unroll
-  for (int i = 0; i < RB; ++i) prow[i] = row_of(16 * i + qn);
+  QueryRows<D, RB> queries;
+  queries.lds = lds.q;
+  queries.Request(a.q, a.q_dtype, row_of);
   float m[RB], l[RB];
   f4v o[RB][D / 16];
-  StreamKeys<FMT, D, PT, RB>(a, a.table + int64_t(first) * a.stride, 0, h, tile0 + wave, kSharedWaves, tile1, shared, prow,
+  StreamKeys<FMT, D, PT, RB>(a, a.table + int64_t(first) * a.stride, 0, h, tile0 + wave, kSharedWaves, tile1, shared, queries,
                              lds.scales[wave], m, l, o);
   // (rows of sequences shorter than the prefix leave partials that nobody reads)
   MergeWaves<D, RB>(a, lds, m, l, o, n_rows - row0, row_of, piece);
