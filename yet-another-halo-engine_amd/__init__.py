@@ -6,6 +6,8 @@ stream to the library. There is no CPU fallback: without the built library the i
 import ctypes as C
 import os
 
+import torch  # first: it brings the HIP runtime that the library binds to (two runtimes in one process share nothing)
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libyahkv.so")
 
@@ -13,6 +15,7 @@ Q8_0, Q4_0, KV_F16, KV8A16 = 8, 4, 16, 816
 KV4A16, K8V4A16, K4V8A16 = 416, 8416, 4816
 _KV8_FORMATS = {(8, 8): KV8A16, (4, 4): KV4A16, (8, 4): K8V4A16, (4, 8): K4V8A16}
 F32, F16, BF16 = 0, 1, 2
+_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
 class YahkvError(RuntimeError):
@@ -70,9 +73,8 @@ class Rows(C.Structure):
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built: run `python __graft_entry__.py build` (hipcc, gfx950)")
-    # torch ships its own HIP runtime (same soname as /opt/rocm's). It must be in the process first, so that the
-    # library binds to that one: two runtimes in one process do not share streams or device memory.
-    import torch  # noqa: F401
+    # torch ships its own HIP runtime (same soname as /opt/rocm's). It is in the process first (imported above), so that the
+    # library binds to that one.
     lib = C.CDLL(LIB_PATH)
     G, P, vp, i32, i32p = C.POINTER(Geometry), C.POINTER(Pools), C.c_void_p, C.c_int32, C.c_void_p
     lib.yahkv_version.restype = C.c_char_p
@@ -257,8 +259,7 @@ def _dp(t):
 
 
 def _dtype_code(t):
-    import torch
-    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
+    return _DTYPES[t.dtype]
 
 
 class F16Pools:
@@ -664,60 +665,63 @@ ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
 ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
 
-def _need(ok, what):
+def _refuse(what):
     """A call the library must not see: tensors whose shape, type or device it would have to take on trust."""
+    raise YahkvError(-1, what)
+
+
+def _need(ok, what):
     if not ok:
-        raise YahkvError(-1, what)
+        _refuse(what)
 
 
 def _ints(t, shape, like, what):
-    import torch
-    _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == like and tuple(t.shape) == tuple(shape),
-          f"{what}: a contiguous int32 tensor of shape {tuple(shape)} on {like} is expected")
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != like or not t.is_contiguous():
+        _refuse(f"{what}: a contiguous int32 tensor of shape {tuple(shape)} on {like} is expected")
 
 
 def _table(t, n_seqs, like, what):
-    import torch
-    _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == like and t.dim() == 2 and t.shape[0] == n_seqs,
-          f"{what}: a contiguous int32 tensor [{n_seqs}][pages] on {like} is expected")
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != n_seqs or t.device != like or not t.is_contiguous():
+        _refuse(f"{what}: a contiguous int32 tensor [{n_seqs}][pages] on {like} is expected")
 
 
-def _run_on(device, call):
+def _run_on(device, call, what):
     """call(stream) on torch's current stream of `device`, with that device current."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        return call(C.c_void_p(torch.cuda.current_stream().cuda_stream))
-    with torch.cuda.device(device):
-        return call(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    if device.type != "cuda":
+        _refuse(f"{what}: tensors on a GPU are expected")
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = call(torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = call(torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        raise YahkvError(status, what)
 
 
 def _out(out, shape, dtype, device, default):
     """The caller's output tensor after a look at it, or a new one."""
-    import torch
     if out is None:
         return torch.empty(shape, dtype=dtype or default, device=device)
-    _need(tuple(out.shape) == tuple(shape) and out.is_contiguous() and out.device == device and
-          dtype in (None, out.dtype) and out.dtype in (torch.float32, torch.float16, torch.bfloat16),
-          f"out: a contiguous tensor of shape {tuple(shape)} on {device} is expected")
+    if out.shape != shape or not out.is_contiguous() or out.device != device or dtype not in (None, out.dtype) or out.dtype not in _DTYPES:
+        _refuse(f"out: a contiguous tensor of shape {tuple(shape)} on {device} is expected")
     return out
 
 
 def _scratch(workspace, need, device):
-    import torch
     if workspace is None:
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == device,
-          "workspace: a contiguous uint8 tensor on the queries' device is expected")
+        return torch.empty(max(need(), 16), dtype=torch.uint8, device=device)
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.device != device:
+        _refuse("workspace: a contiguous uint8 tensor on the queries' device is expected")
     return workspace
 
 
 def _queries(g, q, gate, pools, what):
-    import torch
-    _need(q.dtype in (torch.float32, torch.float16, torch.bfloat16) and q.is_contiguous() and q.dim() == 3 and
-          tuple(q.shape[1:]) == (g.n_q_heads, g.head_dim) and q.shape[0] > 0 and q.device == pools.kq.device,
-          f"{what}: contiguous queries [n_seqs][{g.n_q_heads}][{g.head_dim}] on the pools' device are expected")
-    _need(gate is None or (gate.dtype == torch.float32 and gate.is_contiguous() and gate.shape == q.shape and
-                           gate.device == q.device), f"{what}: gate is f32 of the queries' shape")
+    if (q.dtype not in _DTYPES or q.dim() != 3 or q.shape[1:] != (g.n_q_heads, g.head_dim) or q.shape[0] == 0 or
+            not q.is_contiguous() or q.device != pools.kq.device):
+        _refuse(f"{what}: contiguous queries [n_seqs][{g.n_q_heads}][{g.head_dim}] on the pools' device are expected")
+    if gate is not None and (gate.dtype is not torch.float32 or not gate.is_contiguous() or gate.shape != q.shape or gate.device != q.device):
+        _refuse(f"{what}: gate is f32 of the queries' shape")
 
 
 class Rotary:
@@ -730,7 +734,6 @@ class Rotary:
     def __init__(self, rotary_dim, theta, layout="half", scaling="none", factor=1.0, original_len=0.0, low=1.0, high=32.0,
                  first_dim=0, magnitude=None, normalise=False, eps=1e-6, q_weight=None, k_weight=None, device="cuda:0"):
         import numpy as np
-        import torch
         _need(layout in ROTARY_LAYOUTS and scaling in ROTARY_SCALINGS, f"rotary: layout {layout!r}, scaling {scaling!r}")
         spec = RotarySpec(rotary_dim, ROTARY_SCALINGS[scaling], theta, factor, original_len, low, high)
         turns, own = np.zeros(max(rotary_dim // 2, 1), np.uint64), C.c_float()
@@ -746,17 +749,18 @@ class Rotary:
                                    None if k_weight is None else k_weight.data_ptr())
 
     def check_head(self, head_dim):
-        for w in (self.q_weight, self.k_weight):
-            _need(w is None or w.numel() == head_dim, f"rotary: weights of {head_dim} values are expected")
+        if (self.q_weight is not None and self.q_weight.numel() != head_dim) or (
+                self.k_weight is not None and self.k_weight.numel() != head_dim):
+            _refuse(f"rotary: weights of {head_dim} values are expected")
 
 
 def _rows(t, what):
     """A [n_seqs][n_new][heads][D] tensor, each head's values contiguous, as yahkv_rows."""
-    import torch
-    _need(t.dim() == 4 and t.dtype in (torch.float32, torch.float16, torch.bfloat16) and t.numel() > 0 and
-          (t.stride(3) == 1 or t.shape[3] == 1), f"{what}: rows [n_seqs][n_new][heads][D] with contiguous heads are expected")
-    step = [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]  # (a lone element's stride says nothing)
-    return Rows(t.data_ptr(), _dtype_code(t), t.shape[2], *step)
+    if t.dim() != 4 or t.dtype not in _DTYPES or t.numel() == 0 or t.stride(3) != 1:
+        _refuse(f"{what}: rows [n_seqs][n_new][heads][D] with contiguous heads are expected")
+    n, new, heads, _ = t.shape
+    a, b, c, _ = t.stride()  # (the stride of a dimension of one says nothing)
+    return Rows(t.data_ptr(), _DTYPES[t.dtype], heads, a if n > 1 else 0, b if new > 1 else 0, c if heads > 1 else 0)
 
 
 def _ref(s):
@@ -767,9 +771,9 @@ def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_d
     """Rotates q and / or k, [n_seqs][n_new][heads][D] tensors at any strides of whole 16 bytes (slices of a fused projection),
     token t of sequence s by positions[s][t] (int32). Returns (q_out, k_out), new contiguous tensors of out_dtype (the rows'
     own by default) where none are given; q_out may be q itself. None for rows that were not given."""
-    import torch
     first = q if q is not None else k
-    _need(first is not None and first.dim() == 4, "rotary_rows: q or k [n_seqs][n_new][heads][D]")
+    if first is None or first.dim() != 4:
+        _refuse("rotary_rows: q or k [n_seqs][n_new][heads][D]")
     n_seqs, n_new, _, d = first.shape
     _ints(positions, (n_seqs, n_new), first.device, "positions")
     rotary.check_head(d)
@@ -787,8 +791,8 @@ def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_d
         _need(out.shape == x.shape and out.device == x.device, "rotary_rows: out has the rows' shape")
         args += [_rows(x, "rotary_rows"), _rows(out, "rotary_rows")]
         outs.append(out)
-    _check(_run_on(first.device, lambda st: lib.yahkv_rotary_apply(
-        C.byref(rotary.struct), d, _dp(positions), n_seqs, n_new, *map(_ref, args), st)), "rotary_apply")
+    _run_on(first.device, lambda st: lib.yahkv_rotary_apply(
+        C.byref(rotary.struct), d, _dp(positions), n_seqs, n_new, *map(_ref, args), st), "rotary_apply")
     return tuple(outs)
 
 
@@ -797,10 +801,9 @@ def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None,
     """append() with the rotation of k (and of q, if given) fused in: k / v [n_seqs][n_new][n_kv_heads][D] and q
     [n_seqs][n_new][n_q_heads][D] at any strides of whole 16 bytes, token t of sequence s to slot start_pos[s] + t, turned by
     positions[s][t] (None: by its slot). k_out (f32, contiguous) also receives the rotated K rows. Returns q_out."""
-    import torch
     g = pools.geom
-    _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and tuple(k.shape[2:]) == (g.n_kv_heads, g.head_dim),
-          f"rotary_append: k and v [n_seqs][n_new][{g.n_kv_heads}][{g.head_dim}] are expected")
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.shape[2:] != (g.n_kv_heads, g.head_dim):
+        _refuse(f"rotary_append: k and v [n_seqs][n_new][{g.n_kv_heads}][{g.head_dim}] are expected")
     n_seqs, n_new = k.shape[:2]
     dev = pools.kq.device
     _need(k.device == dev and v.device == dev and rotary.turns.device == dev, "rotary_append: another device than the pools'")
@@ -813,8 +816,8 @@ def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None,
     rotary.check_head(g.head_dim)
     qs = qd = None
     if q is not None:
-        _need(tuple(q.shape) == (n_seqs, n_new, g.n_q_heads, g.head_dim) and q.dtype == k.dtype and q.device == dev,
-              f"rotary_append: q [n_seqs][n_new][{g.n_q_heads}][{g.head_dim}] of k's type is expected")
+        if q.shape != (n_seqs, n_new, g.n_q_heads, g.head_dim) or q.dtype != k.dtype or q.device != dev:
+            _refuse(f"rotary_append: q [n_seqs][n_new][{g.n_q_heads}][{g.head_dim}] of k's type is expected")
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q_out_dtype or torch.float32, device=dev)
         _need(q_out.shape == q.shape and q_out.device == dev, "rotary_append: q_out has q's shape")
@@ -823,9 +826,9 @@ def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None,
     _need(k_out is None or (k_out.dtype == torch.float32 and k_out.is_contiguous() and k_out.shape == k.shape and
                             k_out.device == dev), "rotary_append: k_out is contiguous f32 of k's shape")
     st, ks, vs = pools.struct(), _rows(k, "k"), _rows(v, "v")
-    _check(_run_on(dev, lambda stream: lib.yahkv_rotary_append(
+    _run_on(dev, lambda stream: lib.yahkv_rotary_append(
         C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(start_pos), _dp(n_valid), n_seqs, n_new,
-        C.byref(rotary.struct), _dp(positions), C.byref(ks), C.byref(vs), _ref(qs), _ref(qd), _dp(k_out), stream)),
+        C.byref(rotary.struct), _dp(positions), C.byref(ks), C.byref(vs), _ref(qs), _ref(qd), _dp(k_out), stream),
         "rotary_append")
     return q_out
 
@@ -840,7 +843,6 @@ def decode_attend_shared(pools, table, seq_len, group_first, shared_len, max_sha
     shared_len[j] common tokens, whose whole 64-token tiles lie in the same pages of all their table rows and are read once.
     max_shared_len and max_tail_len are host bounds of shared_len and of what a sequence reads besides. Returns out (f32
     unless out / out_dtype say otherwise)."""
-    import torch
     g = pools.geom
     _queries(g, q, gate, pools, "decode_attend_shared")
     n_seqs, dev = q.shape[0], q.device
@@ -851,13 +853,12 @@ def decode_attend_shared(pools, table, seq_len, group_first, shared_len, max_sha
     _ints(shared_len, (n_groups,), dev, "shared_len")
     _ints(group_first, (n_groups + 1,), dev, "group_first")
     out = _out(out, q.shape, out_dtype, dev, torch.float32)
-    workspace = _scratch(workspace, 0 if workspace is not None else decode_shared_workspace_bytes(
-        g, n_seqs, n_groups, max_shared_len, max_tail_len), dev)
+    workspace = _scratch(workspace, lambda: decode_shared_workspace_bytes(g, n_seqs, n_groups, max_shared_len, max_tail_len), dev)
     st = pools.struct()
-    _check(_run_on(dev, lambda stream: lib.yahkv_decode_attend_shared(
+    _run_on(dev, lambda stream: lib.yahkv_decode_attend_shared(
         C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(seq_len), n_seqs, _dp(group_first), _dp(shared_len),
         n_groups, max_shared_len, max_tail_len, _dp(q), _dtype_code(q), scale, _dp(gate), _dp(out), _dtype_code(out),
-        _dp(workspace), workspace.numel(), stream)), "decode_attend_shared")
+        _dp(workspace), workspace.numel(), stream), "decode_attend_shared")
     return out
 
 
@@ -866,10 +867,9 @@ def decode_weights_workspace_bytes(g, n_seqs, max_seq_len):
 
 
 def _weight_rows(w, g, n_seqs, least, device, what):
-    import torch
-    _need(w.dtype == torch.float32 and w.is_contiguous() and w.device == device and w.dim() == 3 and
-          tuple(w.shape[:2]) == (n_seqs, g.n_kv_heads) and w.shape[2] >= least,
-          f"{what}: contiguous f32 [{n_seqs}][{g.n_kv_heads}][at least {least}] on {device} is expected")
+    if (w.dtype is not torch.float32 or not w.is_contiguous() or w.device != device or w.dim() != 3 or
+            w.shape[:2] != (n_seqs, g.n_kv_heads) or w.shape[2] < least):
+        _refuse(f"{what}: contiguous f32 [{n_seqs}][{g.n_kv_heads}][at least {least}] on {device} is expected")
 
 
 def decode_attend_weights(pools, table, seq_len, max_seq_len, q, scale, weights_out, weights_in=None, decay=1.0, gate=None,
@@ -877,7 +877,6 @@ def decode_attend_weights(pools, table, seq_len, max_seq_len, q, scale, weights_
     """decode_attend() that also leaves weights_out[s][h][t] = decay * weights_in[s][h][t] + the softmax weights of key t over
     kv head h's query heads, f32 [n_seqs][n_kv_heads][>= max_seq_len]; weights_in None: zeros; it may be weights_out.
     Returns out (f32 unless out / out_dtype say otherwise)."""
-    import torch
     g = pools.geom
     _queries(g, q, gate, pools, "decode_attend_weights")
     n_seqs, dev = q.shape[0], q.device
@@ -887,12 +886,12 @@ def decode_attend_weights(pools, table, seq_len, max_seq_len, q, scale, weights_
     _need(weights_in is None or (weights_in.shape == weights_out.shape and weights_in.dtype == torch.float32 and
                                  weights_in.is_contiguous() and weights_in.device == dev), "weights_in: as weights_out")
     out = _out(out, q.shape, out_dtype, dev, torch.float32)
-    workspace = _scratch(workspace, 0 if workspace is not None else decode_weights_workspace_bytes(g, n_seqs, max_seq_len), dev)
+    workspace = _scratch(workspace, lambda: decode_weights_workspace_bytes(g, n_seqs, max_seq_len), dev)
     st = pools.struct()
-    _check(_run_on(dev, lambda stream: lib.yahkv_decode_attend_weights(
+    _run_on(dev, lambda stream: lib.yahkv_decode_attend_weights(
         C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(seq_len), n_seqs, max_seq_len, _dp(q), _dtype_code(q),
         scale, _dp(gate), _dp(out), _dtype_code(out), _dp(weights_in), _dp(weights_out), weights_out.shape[2], decay,
-        _dp(workspace), workspace.numel(), stream)), "decode_attend_weights")
+        _dp(workspace), workspace.numel(), stream), "decode_attend_weights")
     return out
 
 
@@ -900,7 +899,6 @@ def evict_select(g, seq_len, max_seq_len, weights, budget, sink=0, recent=0, kep
     """The positions each kv head keeps of a sequence cut to `budget` tokens: the first `sink`, the last `recent`, and of the
     others the heaviest (ties: the lowest). Returns (kept int32 [n_seqs][n_kv_heads][budget], rising, -1 behind the last;
     n_kept int32 [n_seqs])."""
-    import torch
     _need(seq_len.dim() == 1 and seq_len.is_cuda, "seq_len: lengths on the GPU")
     n_seqs, dev = seq_len.shape[0], seq_len.device
     _ints(seq_len, (n_seqs,), dev, "seq_len")
@@ -911,9 +909,9 @@ def evict_select(g, seq_len, max_seq_len, weights, budget, sink=0, recent=0, kep
         n_kept = torch.empty(n_seqs, dtype=torch.int32, device=dev)
     _ints(kept, (n_seqs, g.n_kv_heads, max(budget, 0)), dev, "kept")
     _ints(n_kept, (n_seqs,), dev, "n_kept")
-    _check(_run_on(dev, lambda stream: lib.yahkv_evict_select(
+    _run_on(dev, lambda stream: lib.yahkv_evict_select(
         C.byref(g), _dp(seq_len), n_seqs, max_seq_len, _dp(weights), weights.shape[2], budget, sink, recent, _dp(kept),
-        _dp(n_kept), stream)), "evict_select")
+        _dp(n_kept), stream), "evict_select")
     return kept, n_kept
 
 
@@ -933,10 +931,10 @@ def evict_compact(pools, table, kept, n_kept, dst_table, weights_in=None, weight
     if weights_out is not None:
         _weight_rows(weights_out, g, n_seqs, budget, dev, "weights_out")
     st = pools.struct()
-    _check(_run_on(dev, lambda stream: lib.yahkv_evict_compact(
+    _run_on(dev, lambda stream: lib.yahkv_evict_compact(
         C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(kept), _dp(n_kept), n_seqs, budget, _dp(dst_table),
         dst_table.shape[1], _dp(weights_in), 0 if weights_in is None else weights_in.shape[2], _dp(weights_out),
-        0 if weights_out is None else weights_out.shape[2], stream)), "evict_compact")
+        0 if weights_out is None else weights_out.shape[2], stream), "evict_compact")
 
 
 # ---- kv8a16: the reference's own KV format (yahkv_kv8_*) --------------------------------------------------------------
