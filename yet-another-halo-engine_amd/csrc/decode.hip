@@ -1305,7 +1305,8 @@ int LaunchPart(const DecodeArgs& a, hipStream_t st) {
   }
 #define YAHKV_LAUNCH_PART(FF, DD, PP)                                                                          \
   do {                                                                                                         \
-    if (a.scores != nullptr) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 0, true>), grid, dim3(64 * kWavesPerGroup), 0, st, a); \
+    if (a.scores != nullptr && a.wg_partials) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 2, true>), grid, dim3(64 * kWavesPerGroup), 0, st, a); \
+    else if (a.scores != nullptr) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 0, true>), grid, dim3(64 * kWavesPerGroup), 0, st, a); \
     else if (a.fused) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 1>), grid, dim3(64 * kWavesPerGroup), 0, st, a);           \
     else if (a.wg_partials) hipLaunchKernelGGL((DattnPart<FF, DD, PP, 2>), grid, dim3(64 * kWavesPerGroup), 0, st, a); \
     else hipLaunchKernelGGL((DattnPart<FF, DD, PP, 0>), grid, dim3(64 * kWavesPerGroup), 0, st, a);                    \
@@ -1492,11 +1493,15 @@ extern "C" int yahkv_decode_attend(const yahkv_geometry* g, const yahkv_pools* p
 }
 
 namespace {
-// Two-dispatch form with a partial per wave (the weighing part kernel has no other), and for a batch of few tiles chunks of
-// one tile per wave.
-yahkv_decode_options WeighOptions() {
+// The two-dispatch forms (the whole-tile kernel does not weigh). A batch of at most four tiles per wave is cut into chunks of
+// one tile per wave, a pair's change costs nothing, and a workgroup leaves one partial of its last pair (one 32K sequence:
+// merge 17.6 -> 8 us); a larger one leaves a partial per wave.
+yahkv_decode_options WeighOptions(const Geom& m, int32_t n_seqs, int32_t max_seq_len) {
+  const int64_t tiles = (int64_t(max_seq_len) + kTile - 1) / kTile * n_seqs * m.n_kv;
+  const bool small = tiles <= int64_t(ComputeUnits()) * kWavesPerGroup * 4;
   yahkv_decode_options o{};
-  o.wg_partials = 2, o.min_chunk_tiles = kWavesPerGroup;
+  o.wg_partials = small ? 1 : 2;
+  if (small) o.min_chunk_tiles = kWavesPerGroup, o.pair_cost = -1;
   return o;
 }
 struct WeighPlan {
@@ -1504,7 +1509,7 @@ struct WeighPlan {
   int32_t score_stride;
 };
 WeighPlan MakeWeighPlan(const Geom& m, int32_t n_seqs, int32_t max_seq_len) {
-  const yahkv_decode_options o = WeighOptions();
+  const yahkv_decode_options o = WeighOptions(m, n_seqs, max_seq_len);
   WeighPlan p;
   p.part = Align(MakePlan(m, n_seqs, max_seq_len, MakeTuning(&o)).bytes);
   p.score_stride = (max_seq_len + kTile - 1) / kTile * kTile;
@@ -1534,7 +1539,7 @@ extern "C" int yahkv_decode_attend_weights(const yahkv_geometry* g, const yahkv_
   if (max_seq_len > kMaxWeighLen) return YAHKV_ERR_SHAPE;
   if (const int st = CheckPartArgs(g, pools, page_table, q, q_dtype)) return st;
   const Geom m = MakeGeom(*g);
-  const yahkv_decode_options o = WeighOptions();
+  const yahkv_decode_options o = WeighOptions(m, n_seqs, max_seq_len);
   DecodeArgs a;
   if (const int st = Prepare(m, page_table_stride, seq_len, n_seqs, max_seq_len, workspace, workspace_bytes, &o, &a)) return st;
   const WeighPlan p = MakeWeighPlan(m, n_seqs, max_seq_len);
