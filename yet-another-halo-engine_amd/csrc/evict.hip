@@ -29,9 +29,13 @@ struct SelectArgs {
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kOwn = 32;                           // keys of a thread at most, consecutive ones, in LDS rows of 33 words
 constexpr int kSegment = kOwn * kSelectThreads;    // (all banks in use); longer rows go through LDS segment by segment
-constexpr int kBins = 2048, kListed = 4096;
+constexpr int kBins = 2048, kListed = 4096, kStaged = 2 * kListed;
 
-__device__ __forceinline__ uint32_t WeightKey(float w) { return w > 0.0f ? __builtin_bit_cast(uint32_t, w) : 0u; }
+// Keys as the passes see them, without a question about positions: a weight's bits + 1 (1 .. 0x7F800001), all ones for a
+// position that is kept whatever it weighs, 0 for none.
+constexpr uint32_t kAlways = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t WeightKey(float w) { return w > 0.0f ? __builtin_bit_cast(uint32_t, w) + 1u : 1u; }
+__device__ __forceinline__ bool Weighed(uint32_t key) { return static_cast<int32_t>(key) > 0; }
 
 __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a) {
   const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
@@ -48,12 +52,17 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
 
   __shared__ uint32_t keys[kSelectThreads * (kOwn + 1)];
   __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t list[kListed];  // the keys that share the threshold's first digit, in any order
+  __shared__ union {
+    uint32_t list[kListed];    // the keys that share the threshold's first digit, in any order
+    uint16_t staged[kStaged];  // kept positions on their way out, within the segment
+  } shared;
+  auto& list = shared.list;
+  auto& staged = shared.staged;
   __shared__ uint32_t totals[kSelectWaves];
   __shared__ uint32_t found[3];       // the digit, how many of the keys that share it are kept, and how many there are
   __shared__ int list_n;
   const int n_segments = (len + kSegment - 1) / kSegment;
-  int lg_own = 0;                     // a thread owns 2^lg_own consecutive keys of a segment
+  int lg_own = 3;                     // a thread owns 2^lg_own consecutive keys of a segment
   while ((kSelectThreads << lg_own) < min(len, kSegment)) ++lg_own;
   const int own = 1 << lg_own;
   int loaded = -1;
@@ -62,23 +71,27 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
     __syncthreads();
     const int base = seg * kSegment, n = min(len - base, kSegment);
     const float* const from = w + base;
-    auto put = [&](int e, float v) { keys[(e >> lg_own) * (kOwn + 1) + (e & (own - 1))] = WeightKey(v); };
+    auto put = [&](int e, float v) {
+      const int t = base + e;
+      keys[(e >> lg_own) * (kOwn + 1) + (e & (own - 1))] = t >= len ? 0u : t < lo || t >= hi ? kAlways : WeightKey(v);
+    };
     const int n4 = (reinterpret_cast<uintptr_t>(from) & 15) == 0 ? n & ~3 : 0;
 #pragma unroll 8
     for (int e = 4 * tid; e < n4; e += 4 * kSelectThreads) {
       const float4 v = *reinterpret_cast<const float4*>(from + e);
       put(e, v.x), put(e + 1, v.y), put(e + 2, v.z), put(e + 3, v.w);
     }
-    for (int e = n4 + tid; e < n; e += kSelectThreads) put(e, from[e]);
+    for (int e = n4 + tid; e < own * kSelectThreads; e += kSelectThreads) put(e, from[min(e, n - 1)]);
     loaded = seg;
     __syncthreads();
   };
-  auto each = [&](int seg, auto f) {  // f(position, key, whether it is weighed) for this thread's keys of a segment, in order
-    const int t0 = seg * kSegment + (tid << lg_own);
-#pragma unroll 4
-    for (int j = 0; j < own; ++j) {
-      const int t = t0 + j;
-      if (t < len) f(t, keys[tid * (kOwn + 1) + j], t >= lo && t < hi);
+  auto each = [&](auto f) {  // f(key, its place among this thread's keys of the segment), in order
+    for (int j0 = 0; j0 < own; j0 += 8) {
+      uint32_t k[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j] = keys[tid * (kOwn + 1) + j0 + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f(k[j], j0 + j);
     }
   };
   // exclusive sum over the threads before this one, and the sum of all
@@ -129,8 +142,8 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
     clear_bins();
     for (int seg = 0; seg < n_segments; ++seg) {
       load(seg);
-      each(seg, [&](int, uint32_t key, bool weighed) {
-        if (weighed) atomicAdd(&bins[key >> 20], 1u);
+      each([&](uint32_t key, int) {
+        if (Weighed(key)) atomicAdd(&bins[key >> 20], 1u);
       });
     }
     find_digit(20, 2047u);
@@ -139,8 +152,8 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
     if (listed) {
       for (int seg = 0; seg < n_segments; ++seg) {
         load(seg);
-        each(seg, [&](int, uint32_t key, bool weighed) {
-          if (weighed && (key & top_mask) == top) list[atomicAdd(&list_n, 1)] = key;
+        each([&](uint32_t key, int) {
+          if (Weighed(key) & ((key & top_mask) == top)) list[atomicAdd(&list_n, 1)] = key;
         });
       }
     }
@@ -157,34 +170,42 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
       } else {  // too many for the list (equal weights): over all keys again
         for (int seg = 0; seg < n_segments; ++seg) {
           load(seg);
-          each(seg, [&](int, uint32_t key, bool weighed) {
-            if (weighed) count(key);
+          each([&](uint32_t key, int) {
+            if (Weighed(key)) count(key);
           });
         }
       }
       find_digit(shift, digits);
     }
   }
-  // Kept: what is not weighed, keys above the threshold, and the first `take` of those equal to it (if nothing is to be taken,
-  // no key is above it either). Counts of both in one word: a segment has 32768 keys at most.
+  // Kept: keys above the threshold, and the first `take` of those equal to it (if nothing is to be taken, what is kept
+  // whatever it weighs). Counts of both in one word: a segment has 32768 keys at most.
+  if (!any) prefix = kAlways - 1;
   uint32_t sure_before = 0, equal_before = 0;
   for (int seg = 0; seg < n_segments; ++seg) {
     load(seg);
     uint32_t mine = 0;
-    each(seg, [&](int, uint32_t key, bool weighed) {
-      mine += !weighed || (any && key > prefix) ? 1u : any && key == prefix ? 0x10000u : 0u;
-    });
+    each([&](uint32_t key, int) { mine += (key > prefix ? 1u : 0u) + (key == prefix ? 0x10000u : 0u); });
     uint32_t all;
     const uint32_t before = scan(mine, &all);
-    uint32_t sure = sure_before + (before & 0xFFFFu), equal = equal_before + (before >> 16);
-    each(seg, [&](int t, uint32_t key, bool weighed) {
-      if (!weighed || (any && key > prefix)) {
-        out[sure + min(equal, take)] = t, ++sure;
-      } else if (any && key == prefix) {
-        if (equal < take) out[sure + equal] = t;
-        ++equal;
-      }
-    });
+    // to their places by way of LDS, 8192 at a time: a thread's own are a few, far apart in time and in memory
+    const uint32_t sure0 = sure_before + (before & 0xFFFFu), equal0 = equal_before + (before >> 16);
+    const uint32_t first = sure_before + min(equal_before, take);
+    const uint32_t last = sure_before + (all & 0xFFFFu) + min(equal_before + (all >> 16), take);
+    for (uint32_t from = first; from < last; from += kStaged) {
+      uint32_t sure = sure0, equal = equal0;
+      each([&](uint32_t key, int j) {
+        const bool above = key > prefix, same = key == prefix;
+        const uint32_t at = sure + min(equal, take) - from;
+        if ((above | (same & (equal < take))) & (at < static_cast<uint32_t>(kStaged)))
+          staged[at] = static_cast<uint16_t>((tid << lg_own) + j);
+        sure += above, equal += same;
+      });
+      __syncthreads();
+      for (uint32_t i = tid; i < min(last - from, static_cast<uint32_t>(kStaged)); i += kSelectThreads)
+        out[from + i] = seg * kSegment + staged[i];
+      __syncthreads();
+    }
     sure_before += all & 0xFFFFu, equal_before += all >> 16;
   }
 }
