@@ -171,6 +171,32 @@ def test_append(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, starts, new, dim, firs
         assert np.array_equal(got[name], want), name
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("fmt,n_kv,hd,pt,dim,first,src", [(8, 4, 256, 64, 256, 0, "bfloat16"), (8, 8, 128, 16, 64, 64, "float16"),
+                                                          (4, 1, 256, 32, 64, 12, "float32"), (4, 2, 128, 64, 128, 0, "bfloat16")])
+def test_chunk_without_rotated_rows_leaves_the_same_pools(yahkv, torch_gpu, fmt, n_kv, hd, pt, dim, first, src, layout):
+    """K turned page by page (no k_out asked for) and token by token: the same operations on the same values, the same bytes,
+    also where a chunk is padded, starts inside a page or runs into the end of the table (the last token owns that slot)."""
+    torch = torch_gpu
+    rng = np.random.default_rng(hd + dim)
+    starts, new, valid = [0, 5, pt - 1, 2 * pt + 3], 77, [77, 9, 60, 77]
+    pages = [(s + new + pt - 1) // pt for s in starts]
+    g = yahkv.geometry(fmt, n_kv, n_kv, hd, pt, sum(pages) + 4)
+    t = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+    table = t(make_tables(rng, pages, g.n_pages))
+    cut = t(np.array([0, 0, 0, table.shape[1] * pt - 50]))
+    x = torch.from_numpy(rng.standard_normal((4, new, 2 * n_kv + 1, hd)).astype(np.float32)).cuda().to(getattr(torch, src))
+    r = make(yahkv, dim, layout, "bands", first_dim=first, normalise=dim != 64, k_weight=torch.rand(hd, device="cuda") + 0.5)
+    for start in (t(starts), cut):
+        a, b = yahkv.DevicePools(g, fill=0x33), yahkv.DevicePools(g, fill=0x33)
+        pos = t(rng.integers(0, 100000, (4, new)))
+        k, v = x[:, :, :n_kv], x[:, :, n_kv:2 * n_kv]
+        yahkv.rotary_append(a, table, start, r, k, v, positions=pos, n_valid=t(valid), k_out=torch.empty(k.shape, device="cuda"))
+        yahkv.rotary_append(b, table, start, r, k, v, positions=pos, n_valid=t(valid))
+        for name in ("kq", "ks", "vq", "vs"):
+            assert torch.equal(getattr(a, name), getattr(b, name)), name
+
+
 def test_append_without_queries_or_norm_equals_rotate_then_append(yahkv, torch_gpu):
     torch = torch_gpu
     rng = np.random.default_rng(4)

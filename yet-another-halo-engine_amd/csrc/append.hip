@@ -220,7 +220,10 @@ constexpr int kPageWaves = 4;
 constexpr int kPageAppendMin = 8;  // tokens per sequence from which a call is treated as a chunk
 // SRC: the source rows' type, known when compiling (as a run-time value it put a three-way branch around every
 // row's conversion).
-template <int FMT, int SRC>
+// TURN: yahkv_rotary_append's chunks: the K rows of a wave's four tokens are normalised and turned before they are quantized.
+// Their cosines and sines are worked out by the wave into LDS, again for every kv head's workgroup (a twentieth of the
+// kernel's instructions; a table for all heads would need memory and a launch of its own).
+template <int FMT, int SRC, bool TURN>
 __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a) {
 #pragma clang fp contract(off)
   const Geom g = a.g;
@@ -261,9 +264,67 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
       if (t >= t_lo && t < t_hi && has) {
         const int tok = token_at(pi * PT + t);
         rv[j] = LoadRaw4(a.v_src, static_cast<size_t>(s * a.v_rows.seq + tok * a.v_rows.token + h * a.v_rows.head) + d0, SRC);
-        if (!a.skip_k) rk[j] = LoadRaw4(a.k_src, ((size_t(s) * a.n_new + tok) * H + h) * D + d0, SRC);
+        if (!a.skip_k) {
+          if constexpr (TURN) rk[j] = LoadRaw4(a.k_src, static_cast<size_t>(s * a.k_rows.seq + tok * a.k_rows.token + h * a.k_rows.head) + d0, SRC);
+          else rk[j] = LoadRaw4(a.k_src, ((size_t(s) * a.n_new + tok) * H + h) * D + d0, SRC);
+        }
       }
     }
+  };
+  __shared__ __align__(16) float lcs[TURN ? kPageWaves : 1][4][TURN ? 128 : 4], lsn[TURN ? kPageWaves : 1][4][TURN ? 128 : 4];
+  float4 wk = {1.0f, 1.0f, 1.0f, 1.0f};
+  if constexpr (TURN)
+    if (a.k_weight != nullptr && has) wk = *reinterpret_cast<const float4*>(a.k_weight + d0);
+  // the K rows of tokens 4 q .. 4 q + 3, normalised and turned (see AppendRows for a lane's part of the rotation)
+  auto turn = [&](int q, float4 (&kx)[4]) {
+    const int rot = a.rotary.rot, half = rot / 2, r0 = d0 - a.rotary.first;
+    const bool turned = has && r0 >= 0 && r0 < rot, inside = a.rotary.layout == YAHKV_ROTARY_INTERLEAVED, first = r0 < half;
+    const int partner = turned && !inside ? (first ? lane + half / 4 : lane - half / 4) : lane;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = min(max(4 * q + j, t_lo), t_hi - 1), tok = token_at(pi * PT + t);
+      const int pos = a.positions != nullptr ? a.positions[static_cast<int64_t>(s) * a.n_new + tok] : start + tok;
+      for (int p = lane; p < half; p += 64) {
+        float c, v;
+        TurnCosSin(pos, a.rotary.turns[p], &c, &v);
+        lcs[wave][j][p] = c * a.rotary.magnitude, lsn[wave][j][p] = v * a.rotary.magnitude;
+      }
+    }
+    if (a.rotary.normalise) {
+      float ss[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss[j] = WaveSum(kx[j].x * kx[j].x + kx[j].y * kx[j].y + kx[j].z * kx[j].z + kx[j].w * kx[j].w);
+      // (lane l works out the reciprocal of row l % 4 for everybody)
+      const float mine = lane & 2 ? (lane & 1 ? ss[3] : ss[2]) : (lane & 1 ? ss[1] : ss[0]);
+      const float inv = 1.0f / sqrtf(mine / static_cast<float>(D) + a.eps);
+      const float i4[4] = {Dpp<0x00>(inv), Dpp<0x55>(inv), Dpp<0xAA>(inv), Dpp<0xFF>(inv)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        kx[j] = float4{(kx[j].x * i4[j]) * wk.x, (kx[j].y * i4[j]) * wk.y, (kx[j].z * i4[j]) * wk.z, (kx[j].w * i4[j]) * wk.w};
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = kx[j];
+      float4 x;
+      if (inside) {
+        const int p = turned ? r0 / 2 : 0;
+        const float2 c = *reinterpret_cast<const float2*>(&lcs[wave][j][p]), sv = *reinterpret_cast<const float2*>(&lsn[wave][j][p]);
+        x = float4{v.x * c.x - v.y * sv.x, v.y * c.x + v.x * sv.x, v.z * c.y - v.w * sv.y, v.w * c.y + v.z * sv.y};
+      } else {
+        const int p = turned ? (first ? r0 : r0 - half) : 0;
+        const float4 c = *reinterpret_cast<const float4*>(&lcs[wave][j][p]);
+        float4 sv = *reinterpret_cast<const float4*>(&lsn[wave][j][p]);
+        if (first) sv = float4{-sv.x, -sv.y, -sv.z, -sv.w};
+        const float px = __shfl(v.x, partner, 64), py = __shfl(v.y, partner, 64);
+        const float pz = __shfl(v.z, partner, 64), pw = __shfl(v.w, partner, 64);
+        x = float4{v.x * c.x + px * sv.x, v.y * c.y + py * sv.y, v.z * c.z + pz * sv.z, v.w * c.w + pw * sv.w};
+      }
+      if (turned) kx[j] = x;
+    }
+    __builtin_amdgcn_wave_barrier();  // (the table is rewritten for the next four tokens)
   };
   if (4 * (t_lo / 4 + wave) < t_hi) request(t_lo / 4 + wave);
   for (int q = t_lo / 4 + wave; 4 * q < t_hi; q += kPageWaves) {
@@ -271,6 +332,7 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
 #pragma unroll
     for (int j = 0; j < 4; ++j) kx[j] = Widen4(rk[j], SRC), vx[j] = Widen4(rv[j], SRC);
     if (4 * (q + kPageWaves) < t_hi) request(q + kPageWaves);
+    if constexpr (TURN) turn(q, kx);
     uint32_t vc[4];
     if constexpr (FMT == 8) {
       // Eight rows are in flight (K and V of four tokens) and a block has eight lanes: lane lb of a block takes row
@@ -422,18 +484,19 @@ int CheckAppend(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t
 namespace {
 // AppendRows for the pools' format and the source rows' type (the kernel is compiled for each pair)
 // AppendPages likewise: one workgroup per (page the chunk touches, kv head, sequence)
+template <bool TURN>
 void LaunchPages(int32_t format, int32_t src_dtype, int32_t n_seqs, int32_t n_new, hipStream_t st, const RopeArgs& a) {
   const dim3 grid(static_cast<unsigned>((n_new + a.g.pt - 2) / a.g.pt + 1), static_cast<unsigned>(a.g.n_kv),
                   static_cast<unsigned>(n_seqs));
   const dim3 block(64 * kPageWaves);
   if (format == YAHKV_Q8_0) {
-    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<8, YAHKV_F32>), grid, block, 0, st, a);
-    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<8, YAHKV_F16>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((AppendPages<8, YAHKV_BF16>), grid, block, 0, st, a);
+    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<8, YAHKV_F32, TURN>), grid, block, 0, st, a);
+    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<8, YAHKV_F16, TURN>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((AppendPages<8, YAHKV_BF16, TURN>), grid, block, 0, st, a);
   } else {
-    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<4, YAHKV_F32>), grid, block, 0, st, a);
-    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<4, YAHKV_F16>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((AppendPages<4, YAHKV_BF16>), grid, block, 0, st, a);
+    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<4, YAHKV_F32, TURN>), grid, block, 0, st, a);
+    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<4, YAHKV_F16, TURN>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((AppendPages<4, YAHKV_BF16, TURN>), grid, block, 0, st, a);
   }
 }
 template <int ROPE>
@@ -464,11 +527,26 @@ int LaunchTurned(RopeArgs a, hipStream_t st) {
   if (n_new >= kPageAppendMin && n_seqs <= 65535) {
     // A chunk: V page by page, as the plain append takes it (whole lines from an image of the page, where the
     // token's workgroup would store V's codes byte by byte into the transposed page), K and the query rows by token.
+    // The general rotation has K page by page as well, unless the caller wants the rotated rows of every token (those that
+    // clamp to a slot another token takes are not visited there), and the query rows by the rows kernel, which has eight
+    // dims a lane and several rows a wave where AppendRows has four and one (5 x 1037 tokens of 32 + 8 heads of 128 dims:
+    // @@).
+    const bool k_pages = MODE == kGeneral && a.k_out == nullptr;
     RopeArgs v = a;
-    v.skip_k = 1;
-    LaunchPages(format, src_dtype, n_seqs, n_new, st, v);
+    v.skip_k = !k_pages;
+    if (k_pages) LaunchPages<true>(format, src_dtype, n_seqs, n_new, st, v);
+    else LaunchPages<false>(format, src_dtype, n_seqs, n_new, st, v);
     if (const int rc = LaunchStatus()) return rc;
     a.skip_v = 1;
+    if constexpr (MODE == kGeneral) {
+      if (a.q_src != nullptr) {
+        if (const int rc = LaunchRotaryRows(a.rotary, m.hd, a.positions, a.start_pos, a.n_valid, n_seqs, n_new, a.q_rows, a.q_out_rows,
+                                            RowsArgs{}, RowsArgs{}, st))
+          return rc;
+        a.q_src = nullptr;
+      }
+      if (k_pages) return YAHKV_OK;
+    }
   }
   int64_t blocks = tokens;
   if (n_new >= 8 * m.pt) {  // a long chunk: a page's tokens to one XCD (see AppendRows)
@@ -494,7 +572,7 @@ extern "C" int yahkv_append(const yahkv_geometry* g, const yahkv_pools* pools, c
   a.src_dtype = src_dtype, a.rotary_dim = 8, a.theta = 1.0f, a.v_rows = DenseRows(a, v_src);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (n_new >= kPageAppendMin && n_seqs <= 65535) {  // a chunk: page by page (the grid's z extent is the batch)
-    LaunchPages(g->format, src_dtype, n_seqs, n_new, st, a);
+    LaunchPages<false>(g->format, src_dtype, n_seqs, n_new, st, a);
     return LaunchStatus();
   }
   const dim3 grid(static_cast<unsigned>(n_seqs) * static_cast<unsigned>(n_new));

@@ -20,6 +20,8 @@ namespace {
 struct ApplyArgs {
   RotaryArgs r;
   const int32_t* positions;
+  const int32_t* start_pos;
+  const int32_t* n_valid;
   int32_t n_new, hd, lanes;  // lanes: lanes of a row, a power of two, at least hd / 8
   int32_t n_rows, rows_per_group;  // rows of a token (query heads, then key heads), and of one workgroup of it
   RowsArgs qs, qd, ks, kd;   // qs.n_heads may be 0
@@ -31,6 +33,7 @@ template <int SRC>
 __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
   const int token = blockIdx.x, s = token / a.n_new, t = token % a.n_new;
   const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = kRowThreads / lanes;
+  if (a.n_valid != nullptr && t >= a.n_valid[s]) return;  // padding row of a short chunk
   const int row_end = min(a.n_rows, static_cast<int>(blockIdx.y + 1) * a.rows_per_group);
   // this lane's two pieces: whole pairs, or dims that pass through
   const int rot = a.r.rot, half = rot / 2, first = a.r.first;
@@ -62,7 +65,7 @@ __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
   request(row_first);  // (asked for before the sines are worked out)
 
   __shared__ __align__(16) float cs[256], sn[256];
-  const int pos = a.positions[static_cast<int64_t>(s) * a.n_new + t];
+  const int pos = a.positions != nullptr ? a.positions[static_cast<int64_t>(s) * a.n_new + t] : a.start_pos[s] + t;
   for (int p = threadIdx.x; p < half; p += kRowThreads) {
     float c, v;
     TurnCosSin(pos, a.r.turns[p], &c, &v);
@@ -113,6 +116,29 @@ __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
 }
 
 }  // namespace
+
+int LaunchRotaryRows(const RotaryArgs& r, int32_t head_dim, const int32_t* positions, const int32_t* start_pos,
+                     const int32_t* n_valid, int32_t n_seqs, int32_t n_new, const RowsArgs& q_src, const RowsArgs& q_dst,
+                     const RowsArgs& k_src, const RowsArgs& k_dst, hipStream_t st) {
+  const int64_t tokens = int64_t(n_seqs) * n_new;
+  ApplyArgs a{};
+  a.r = r, a.positions = positions, a.start_pos = start_pos, a.n_valid = n_valid, a.n_new = n_new, a.hd = head_dim;
+  a.qs = q_src, a.qd = q_dst, a.ks = k_src, a.kd = k_dst, a.n_rows = q_src.n_heads + k_src.n_heads;
+  a.lanes = 1;
+  while (a.lanes < head_dim / 8) a.lanes *= 2;
+  // Few tokens: a token's rows go to several workgroups, each with one round of loads; many: all rows of a token share
+  // one workgroup's sines.
+  const int at_once = kRowThreads / a.lanes * kRowsAtOnce;
+  a.rows_per_group = tokens >= 1024 ? a.n_rows : at_once;
+  const unsigned groups = static_cast<unsigned>((a.n_rows + a.rows_per_group - 1) / a.rows_per_group);
+  const dim3 grid(static_cast<unsigned>(tokens), groups);
+  const int32_t src = q_src.n_heads != 0 ? q_src.dtype : k_src.dtype;
+  if (src == YAHKV_F32) hipLaunchKernelGGL(RotaryRows<YAHKV_F32>, grid, dim3(kRowThreads), 0, st, a);
+  else if (src == YAHKV_F16) hipLaunchKernelGGL(RotaryRows<YAHKV_F16>, grid, dim3(kRowThreads), 0, st, a);
+  else hipLaunchKernelGGL(RotaryRows<YAHKV_BF16>, grid, dim3(kRowThreads), 0, st, a);
+  return LaunchStatus();
+}
+
 }  // namespace yahkv
 
 using namespace yahkv;
@@ -177,19 +203,5 @@ extern "C" int yahkv_rotary_apply(const yahkv_rotary* rotary, int32_t head_dim, 
   }
   const int64_t tokens = int64_t(n_seqs) * n_new, rows = int64_t(a.qs.n_heads) + a.ks.n_heads;
   if (tokens > 0x7FFFFFFF || rows > 65536) return YAHKV_ERR_SHAPE;
-  a.positions = positions, a.n_new = n_new, a.hd = head_dim, a.n_rows = static_cast<int32_t>(rows);
-  a.lanes = 1;
-  while (a.lanes < head_dim / 8) a.lanes *= 2;
-  // Few tokens: a token's rows go to several workgroups, each with one round of loads; many: all rows of a token share
-  // one workgroup's sines.
-  const int at_once = kRowThreads / a.lanes * kRowsAtOnce;
-  a.rows_per_group = tokens >= 1024 ? a.n_rows : at_once;
-  const unsigned groups = static_cast<unsigned>((a.n_rows + a.rows_per_group - 1) / a.rows_per_group);
-  const dim3 grid(static_cast<unsigned>(tokens), groups);
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  const int32_t src = q_src != nullptr ? a.qs.dtype : a.ks.dtype;
-  if (src == YAHKV_F32) hipLaunchKernelGGL(RotaryRows<YAHKV_F32>, grid, dim3(kRowThreads), 0, st, a);
-  else if (src == YAHKV_F16) hipLaunchKernelGGL(RotaryRows<YAHKV_F16>, grid, dim3(kRowThreads), 0, st, a);
-  else hipLaunchKernelGGL(RotaryRows<YAHKV_BF16>, grid, dim3(kRowThreads), 0, st, a);
-  return LaunchStatus();
+  return LaunchRotaryRows(a.r, head_dim, positions, nullptr, nullptr, n_seqs, n_new, a.qs, a.qd, a.ks, a.kd, static_cast<hipStream_t>(stream));
 }

@@ -22,14 +22,21 @@ struct RowsArgs {
 
 // cos and sin of the angle pos * f, f in turns as a 0.64 binary fraction: the product modulo 2^64 is the angle's exact
 // fraction of a turn (f itself is rounded to 2^-65 turns: at position 2^31 that is 2^-34 turns). Its top 32 bits split
-// into a quarter turn and a remainder of at most an eighth of a turn either way, which f32 holds to 2^-24 relative.
+// into a quarter turn and a remainder x of at most an eighth of a turn either way, which f32 holds to 2^-24 relative; on
+// |x| <= pi / 4 the Taylor sums up to x^9 and x^8 are short of sine and cosine by x^11 / 11! < 2^-28 and x^10 / 10! < 2^-25.
 __device__ __forceinline__ void TurnCosSin(int pos, uint64_t turns, float* c, float* s) {
-  const uint64_t angle = static_cast<uint64_t>(static_cast<int64_t>(pos)) * turns;
-  const uint32_t top = static_cast<uint32_t>(angle >> 32);
+  const uint32_t p = static_cast<uint32_t>(pos), lo = static_cast<uint32_t>(turns), hi = static_cast<uint32_t>(turns >> 32);
+  // the high word of the product's low 64 bits, pos as a signed number
+  const uint32_t top = __umulhi(p, lo) + p * hi - (pos < 0 ? lo : 0u);
   const uint32_t quarter = (top + 0x20000000u) >> 30;
-  const int32_t rest = static_cast<int32_t>(top - (quarter << 30));
-  float sv, cv;
-  sincospif(static_cast<float>(rest) * 0x1p-31f, &sv, &cv);  // half turns
+  const float x = static_cast<float>(static_cast<int32_t>(top - (quarter << 30))) * 0x1.921fb6p-30f;  // 2 pi / 2^32
+  const float x2 = x * x;
+  float sv = __builtin_fmaf(x2, 1.0f / 362880.0f, -1.0f / 5040.0f);
+  sv = __builtin_fmaf(x2, sv, 1.0f / 120.0f), sv = __builtin_fmaf(x2, sv, -1.0f / 6.0f);
+  sv = __builtin_fmaf(x2 * x, sv, x);
+  float cv = __builtin_fmaf(x2, 1.0f / 40320.0f, -1.0f / 720.0f);
+  cv = __builtin_fmaf(x2, cv, 1.0f / 24.0f), cv = __builtin_fmaf(x2, cv, -0.5f);
+  cv = __builtin_fmaf(x2, cv, 1.0f);
   const float a = quarter & 1 ? sv : cv, b = quarter & 1 ? cv : sv;
   *c = quarter == 1 || quarter == 2 ? -a : a;
   *s = quarter >= 2 ? -b : b;
@@ -55,6 +62,12 @@ inline int CheckRows(const yahkv_rows* r, RowsArgs* a) {
   *a = RowsArgs{r->data, r->dtype, r->n_heads, r->seq_stride, r->token_stride, r->head_stride};
   return YAHKV_OK;
 }
+
+// The rows kernel (rotary.hip): q and / or k rows (n_heads 0: none) of n_seqs x n_new tokens, turned by positions[s][t] or,
+// where that is null, by start_pos[s] + t; rows at or past n_valid[s] (null: n_new) are left alone. Arguments are checked.
+int LaunchRotaryRows(const RotaryArgs& r, int32_t head_dim, const int32_t* positions, const int32_t* start_pos,
+                     const int32_t* n_valid, int32_t n_seqs, int32_t n_new, const RowsArgs& q_src, const RowsArgs& q_dst,
+                     const RowsArgs& k_src, const RowsArgs& k_dst, hipStream_t st);
 
 }  // namespace yahkv
 
