@@ -444,14 +444,16 @@ int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* pools, const
  * [n_groups + 1], rising from 0 to n_seqs), and their page-table rows name the same pages for the prefix's first
  * 64 * floor(shared_len[j] / 64) tokens (device int32 [n_groups]; forks share a prefix's full pages): these are read
  * through the row of the group's first sequence, the rest of every sequence through its own row. A sequence
- * shorter than those tiles is read through its own row alone (max_tail_len has to cover it); one of length 0 gives zeros. Results are those of yahkv_decode_attend up to the order of the sums
+ * shorter than those tiles is read through its own row alone (max_tail_len has to cover it); one of length 0 gives zeros.
+ * Results are those of yahkv_decode_attend up to the order of the sums
  * (both within 2e-3 of exact arithmetic on the dequantized K / V; a 16-bit out adds its own rounding).
  *   q, gate    as yahkv_decode_attend
  *   out        [n_seqs][n_q_heads][D] of out_dtype (F32, F16 or BF16), 16-byte aligned
  *   max_shared_len, max_tail_len  host bounds: of shared_len[] (a longer prefix is cut to the bound and the rest counts as
  *              tail) and of the tokens any sequence reads through its own row (more are cut off, as lengths above
  *              max_seq_len are elsewhere)
- * softmax_scale > 0. Three dispatches: prefixes, tails (yahkv_decode_part), the merge. */
+ * softmax_scale > 0. Two dispatches, the partials of prefixes and tails and their merge, or three: tails that fill the GPU
+ * have one of their own. */
 size_t yahkv_decode_shared_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t n_groups, int32_t max_shared_len,
                                            int32_t max_tail_len);
 int yahkv_decode_attend_shared(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,

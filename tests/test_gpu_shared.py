@@ -104,6 +104,29 @@ def test_lengths_and_groups(yahkv, torch_gpu, groups):
     check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, gate=gate, **a), want, torch.float32)
 
 
+@pytest.mark.parametrize("fmt,pt", [(8, 64), (8, 32), (8, 16), (4, 64), (4, 32), (4, 16)])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(24, 4, 256), (32, 8, 128)])
+def test_bounds_of_a_large_call(yahkv, torch_gpu, n_q, n_kv, hd, fmt, pt):
+    """The host bounds of a long context choose as many row blocks a wave as registers hold, and tails in a launch of their
+    own, whatever the lengths on the device are."""
+    torch = torch_gpu
+    groups = [(640, [650 + 7 * i for i in range(20)]), (0, [3]), (200, [100, 200, 330])]
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, fmt, n_q, n_kv, hd, pt, groups, fmt + pt + hd)
+    a.update(max_shared_len=65536, max_tail_len=40000)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), hd ** -0.5)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=hd ** -0.5, **a), want, torch.float32)
+
+
+def test_more_groups_than_lanes(yahkv, torch_gpu):
+    torch = torch_gpu
+    groups = [(64 * (i % 4), [64 * (i % 4) + 1 + i] * (1 + i % 3)) for i in range(131)]
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 4, 2, 128, 64, groups, 131)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), 0.1)
+    for bound in (192, 65536):
+        a["max_shared_len"] = bound
+        check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **a), want, torch.float32)
+
+
 def test_bounds_clamp(yahkv, torch_gpu):
     """A prefix beyond max_shared_len counts as tail; a shared_len that is negative or past the table is cut to it."""
     torch = torch_gpu

@@ -530,7 +530,7 @@ int LaunchTurned(RopeArgs a, hipStream_t st) {
     // The general rotation has K page by page as well, unless the caller wants the rotated rows of every token (those that
     // clamp to a slot another token takes are not visited there), and the query rows by the rows kernel, which has eight
     // dims a lane and several rows a wave where AppendRows has four and one (5 x 1037 tokens of 32 + 8 heads of 128 dims:
-    // @@).
+    // 101 -> 57 us).
     const bool k_pages = MODE == kGeneral && a.k_out == nullptr;
     RopeArgs v = a;
     v.skip_k = !k_pages;

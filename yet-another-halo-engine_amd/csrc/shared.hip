@@ -4,7 +4,8 @@
 // Attention splits over any partition of the keys: with m a reference point, l = sum 2^(s_t - m) and o = sum 2^(s_t - m)
 // V_t of each part, the whole is (sum 2^(m_p - M) o_p) / (sum 2^(m_p - M) l_p). The prefix's part of a group's rows is a
 // matrix product with many rows (sequences x query heads of a kv head); the tails have one sequence's query heads each.
-// `SharedPart` leaves partials of both in one launch, `SharedMerge` puts them together.
+// `SharedPart` leaves partials of both, in one launch or (tails that fill the chip by themselves) two, `SharedMerge` puts
+// them together.
 //
 // SharedPart: a wave takes 16 RB query rows and 64-key tiles, everything transposed (keys along MFMA rows, query rows along
 // lanes), and works alone: codes go from memory to its registers, are decoded there and feed the products directly.
@@ -18,8 +19,12 @@
 // time to arrive, without a barrier anywhere in the loop. Decoding is packed f16 arithmetic, perm, add, multiply for two
 // values, the product d * code rounded once and saturated at the largest finite f16 (SetSaturation).
 //
-// What bounds it: with 16 or 32 rows the reads; with 48 the vector units (64 decodes of 14 instructions a tile and wave,
-// against 192 matrix instructions of 16 cycles). 48 rows is what fits: accumulators 192, queries 96, codes 128 registers.
+// What bounds it: with few rows the reads and a workgroup's beginning and end (12 query rows on 32K keys of 4 x 256 dims: 23
+// us, 71 MB); with three row blocks of 256 dims the vector unit, which issues 1470 instructions of 4 cycles for a tile's 192
+// matrix instructions of 16 and is busy with 900 of them decoding (384 rows x 32K keys: 97 us, 0.53 PFLOP/s, 4.5 us a tile of
+// each wave, of which a matrix product at this card's rate would take 2.7). Three row blocks are what fits: accumulators 192
+// registers, queries 96, codes 64, scores 48. Decoding once for four waves of other rows, through LDS, brings a tile to 3.2 us, but
+// then no two waves share rows, and writing four times the partials and reading them again takes all of it back.
 #include "codes.hpp"
 #include "common.hpp"
 #include "decode_cut.hpp"
@@ -113,6 +118,14 @@ __device__ __forceinline__ void SetSaturation(const uint4 k, const uint4 v) {
   __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, __builtin_amdgcn_readfirstlane(large && finite ? 1 : 0));
 }
 
+// A barrier behind LDS accesses alone: __syncthreads() would wait for the loads on their way in as well.
+__device__ __forceinline__ void LdsBarrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int D>
 struct WaveScales {  // a tile's scales in LDS, [key][block] and [block][key]
   _Float16 k[kTile * D / 32], v[D / 32 * kTile];
@@ -149,20 +162,58 @@ struct QueryRows {
 #pragma unroll
       for (int j = 0; j < PER; ++j) put(j, ConvertQ8(raw[j], YAHKV_F32));
     }
-    // (a bare barrier behind the LDS writes: __syncthreads() would wait for the codes on their way in as well)
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    LdsBarrier();
   }
   __device__ __forceinline__ h8v At(int row, int d) const { return *reinterpret_cast<const h8v*>(&lds[row][d]); }
 };
+
+// Numerators of one row block's tile: this lane's 16 keys 16 jg + 4 kt + r of its row, scores st in, second operand pv out.
+template <int D>
+__device__ __forceinline__ void Numerators(const f4v (&st)[4], float sscale, float& m, float& l, f4v (&o)[D / 16], h8v (&pv)[2]) {
+  constexpr int NDT = D / 16;
+  float mx = fmaxf(st[0][0], st[0][1]);
+  mx = fmaxf(fmaxf(mx, st[0][2]), st[0][3]);
+#pragma unroll
+  for (int kt = 1; kt < 4; ++kt) mx = fmaxf(fmaxf(mx, st[kt][0]), st[kt][1]), mx = fmaxf(fmaxf(mx, st[kt][2]), st[kt][3]);
+  mx = OverLaneGroups(mx, [](float x, float y) { return fmaxf(x, y); }) * sscale;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m + (kBias + kSlack)) != 0, 0)) {
+    const float mn = mx > m + (kBias + kSlack) ? __builtin_ceilf(mx) - kBias : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    m = mn, l *= alpha;
+    // (the rescaled accumulators go back through a matrix instruction with zero factors: that keeps them in the
+    // accumulation registers on this path as on the common one)
+    const h8v zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      f4v x = o[dt];
+      asm volatile("" : "+a"(x));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] *= alpha;
+      o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zero, zero, x, 0, 0, 0);
+    }
+  }
+  const h2v one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+  uint32_t w[2][4];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    float p[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][r], sscale, -m));
+    const h2v p0 = {static_cast<_Float16>(p[0]), static_cast<_Float16>(p[1])};
+    const h2v p1 = {static_cast<_Float16>(p[2]), static_cast<_Float16>(p[3])};
+    // (the sum is of the rounded numerators, as the second product's is)
+    l = __builtin_amdgcn_fdot2(p0, one, l, false), l = __builtin_amdgcn_fdot2(p1, one, l, false);
+    w[kt / 2][2 * (kt % 2)] = __builtin_bit_cast(uint32_t, p0), w[kt / 2][2 * (kt % 2) + 1] = __builtin_bit_cast(uint32_t, p1);
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) pv[s] = __builtin_bit_cast(h8v, uint4{w[s][0], w[s][1], w[s][2], w[s][3]});
+}
 
 // Tiles tile0, tile0 + step, .. below tile1 of the sequence behind table row `row`, from key `origin` on, `n_keys` keys in
 // all (those at or past it are masked), against RB row blocks: reference points, this lane's part of the sums, accumulators.
 // All four waves of the workgroup call it together (the queries go through LDS behind one barrier); a wave without a tile
 // loads one all the same.
-template <int FMT, int D, int PT, int RB>
+template <int FMT, int D, int PT, int RB, bool TWO>
 __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* row, int origin, int h, int tile0, int step,
                                            int tile1, int n_keys, QueryRows<D, RB>& queries, WaveScales<D>& lds, float (&m)[RB],
                                            float (&l)[RB], f4v (&o)[RB][D / 16]) {
@@ -189,58 +240,52 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
     for (int j = 1; j < PPT; ++j) p = key / PT == j ? pg[j] : p;
     return size_t(p) * H + h;
   };
-  // codes on their way in. Where accumulators and queries leave room, K and V have registers of their own and a load about
-  // a tile's time to arrive; else (three row blocks of 256 dims) they share one set: a V load goes out as soon as a K
-  // load's codes are decoded, and the next tile's K loads as V's are.
-  constexpr bool kOneSet = RB * D > 2 * 256;
-  constexpr int NK = 4 * NP;
-  static_assert(!kOneSet || NK == NV, "a V load for every K load");
-  uint4 kset[NK], vset[kOneSet ? 1 : NV], ksr, vsr;
-  auto kc = [&](int j) -> uint4& { return kset[j]; };
-  auto vc = [&](int j) -> uint4& {
-    if constexpr (kOneSet) return kset[j];
-    else return vset[j];
-  };
+  // Codes on their way in: a tile's K loads, then its V loads, then the next tile's, `kDepth` of them at a time. As soon as
+  // the codes of one are decoded its register is asked for the one kDepth later. (Eight where 256 registers have to do for
+  // accumulators of 256 dims a row block: 32K keys x 12 rows 23 us with two workgroups a CU, 31 with one and 32 loads.)
+  constexpr int NK = 4 * NP, NL = NK + NV, kMost = TWO && Q8 && RB * D == 256 ? 8 : 16, kDepth = NL < kMost ? NL : kMost;
+  static_assert(NL % kDepth == 0, "the same registers in every tile");
+  uint4 codes[kDepth], ksr, vsr;
   constexpr uint32_t KB = Q8 ? 32 : 16;
   // Where a tile is one page, through a buffer resource of the (page, kv head) region: scalar base and offsets, one lane
-  // offset for all loads. Codes that several row blocks read are left to the caches, others go by the non-temporal hint.
-  constexpr int kHint = RB == 3 ? 0 : kStreamed;
+  // offset for all loads.
   auto read = [&](const uint8_t* base, uint32_t lane_off, uint32_t off) -> uint4 {
     if constexpr (PPT == 1) {
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7fffffff, 0x00020000);
-      return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, off, kHint));
+      return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane_off, off, 0));
     } else {
-      const uint4* at = reinterpret_cast<const uint4*>(base + lane_off + off);
-      return kHint != 0 ? StreamLoad(at) : *at;
+      return *reinterpret_cast<const uint4*>(base + lane_off + off);
     }
   };
   const int key0 = 16 * (qn / 4) + qn % 4;  // this lane's key of key tile 0
   const uint32_t k_off = ((Q8 ? jg >> 1 : jg) * PT + key0 % PT) * KB + (Q8 ? 16 * (jg & 1) : 0);
   const uint32_t v_off = qn * PT + 16 * jg % PT;
   auto load_k = [&](const int (&pg)[PPT], int j) {  // load j = NP kt + p (the four key tiles of a lane lie in one page)
-    kc(j) = read(a.pools.kq + page_head(pg, key0) * (NB * PT * KB), k_off, (j % NP * (Q8 ? 2 : 4) * PT + 4 * (j / NP)) * KB);
+    codes[j % kDepth] = read(a.pools.kq + page_head(pg, key0) * (NB * PT * KB), k_off, (j % NP * (Q8 ? 2 : 4) * PT + 4 * (j / NP)) * KB);
   };
   auto load_v = [&](const int (&pg)[PPT], int j) {  // q8_0: dim 16 j + qn; q4_0: byte row qn of block j
-    vc(j) = read(a.pools.vq + page_head(pg, 16 * jg) * (Q8 ? D * PT : NB * 16 * PT), v_off, 16 * j * PT);
+    codes[(NK + j) % kDepth] = read(a.pools.vq + page_head(pg, 16 * jg) * (Q8 ? D * PT : NB * 16 * PT), v_off, 16 * j * PT);
   };
   auto load_scales = [&](const int (&pg)[PPT]) {  // lane: 8 K scales of the tile in [key][block] order, 8 V scales in [block][key]
     ksr = vsr = uint4{0u, 0u, 0u, 0u};
     if (lane < NB * 8) {
       const int key = lane * 8 / NB, chunk = lane % 8;
-      ksr = StreamLoad(reinterpret_cast<const uint4*>(a.pools.ks + (page_head(pg, key) * PT + key % PT) * NB + lane * 8 % NB));
-      vsr = StreamLoad(reinterpret_cast<const uint4*>(a.pools.vs + (page_head(pg, 8 * chunk) * NB + lane / 8) * PT + 8 * chunk % PT));
+      ksr = *reinterpret_cast<const uint4*>(a.pools.ks + (page_head(pg, key) * PT + key % PT) * NB + lane * 8 % NB);
+      vsr = *reinterpret_cast<const uint4*>(a.pools.vs + (page_head(pg, 8 * chunk) * NB + lane / 8) * PT + 8 * chunk % PT);
     }
   };
 
   int pgc[PPT], pgn[PPT];
+  auto load = [&](int j) {  // load j of the tile of pgc, and on into that of pgn
+    if (j < NK) load_k(pgc, j);
+    else if (j < NL) load_v(pgc, j - NK);
+    else if (j < NL + NK) load_k(pgn, j - NL);
+    else load_v(pgn, j - NL - NK);
+  };
   load_pages(tile0, pgn);
   load_scales(pgn);
 #pragma unroll
-  for (int j = 0; j < NK; ++j) load_k(pgn, j);
-  if constexpr (!kOneSet) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) load_v(pgn, j);
-  }
+  for (int j = 0; j < kDepth; ++j) load(NL + j);
   // the queries, which were asked for before all this: through LDS into the first product's operands
   queries.Stage(a.q_dtype);
   h8v qb[RB][KS];
@@ -291,15 +336,14 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
       for (int p = 0; p < NP; ++p) {
         const _Float16 d = lds.k[key * NB + (Q8 ? 2 * p + (jg >> 1) : 4 * p + jg)];
         const h8v d8 = {d, d, d, d, d, d, d, d};
-        const uint4 c = kc(NP * kt + p);
+        const uint4 c = codes[(NP * kt + p) % kDepth];
         h8v ka[SP];
         if constexpr (Q8) {
           ka[0] = Codes8(c.x, c.y), ka[1] = Codes8(c.z, c.w);
         } else {
           ka[0] = NibblesLo8(c.x, c.y), ka[1] = NibblesLo8(c.z, c.w), ka[2] = NibblesHi8(c.x, c.y), ka[3] = NibblesHi8(c.z, c.w);
         }
-        if constexpr (kOneSet) load_v(pgc, NP * kt + p);
-        else load_k(pgn, NP * kt + p);
+        load(NP * kt + p + kDepth);
 #pragma unroll
         for (int sub = 0; sub < SP; ++sub) {
           ka[sub] *= d8;
@@ -310,7 +354,6 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    // ---- numerators: this lane's 16 keys 16 jg + 4 kt + r of its row
     h8v pv[RB][2];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
@@ -321,42 +364,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
           for (int r = 0; r < 4; ++r)
             if (tile * kTile + 16 * jg + 4 * kt + r >= n_keys) st[i][kt][r] = kNegMax;
       }
-      float mx = fmaxf(st[i][0][0], st[i][0][1]);
-      mx = fmaxf(fmaxf(mx, st[i][0][2]), st[i][0][3]);
-#pragma unroll
-      for (int kt = 1; kt < 4; ++kt) mx = fmaxf(fmaxf(mx, st[i][kt][0]), st[i][kt][1]), mx = fmaxf(fmaxf(mx, st[i][kt][2]), st[i][kt][3]);
-      mx = OverLaneGroups(mx, [](float x, float y) { return fmaxf(x, y); }) * sscale;
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m[i] + (kBias + kSlack)) != 0, 0)) {
-        const float mn = mx > m[i] + (kBias + kSlack) ? __builtin_ceilf(mx) - kBias : m[i];
-        const float alpha = __builtin_amdgcn_exp2f(m[i] - mn);
-        m[i] = mn, l[i] *= alpha;
-        // (the rescaled accumulators go back through a matrix instruction with zero factors: that keeps them in the
-        // accumulation registers on this path as on the common one)
-        const h8v zero = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) {
-          f4v x = o[i][dt];
-          asm volatile("" : "+a"(x));
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] *= alpha;
-          o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zero, zero, x, 0, 0, 0);
-        }
-      }
-      const h2v one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-      uint32_t w[2][4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        float p[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][kt][r], sscale, -m[i]));
-        const h2v p0 = {static_cast<_Float16>(p[0]), static_cast<_Float16>(p[1])};
-        const h2v p1 = {static_cast<_Float16>(p[2]), static_cast<_Float16>(p[3])};
-        // (the sum is of the rounded numerators, as the second product's is)
-        l[i] = __builtin_amdgcn_fdot2(p0, one, l[i], false), l[i] = __builtin_amdgcn_fdot2(p1, one, l[i], false);
-        w[kt / 2][2 * (kt % 2)] = __builtin_bit_cast(uint32_t, p0), w[kt / 2][2 * (kt % 2) + 1] = __builtin_bit_cast(uint32_t, p1);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) pv[i][s] = __builtin_bit_cast(h8v, uint4{w[s][0], w[s][1], w[s][2], w[s][3]});
+      Numerators<D>(st[i], sscale, m[i], l[i], o[i], pv[i]);
     }
     // ---- O^T
 #pragma unroll
@@ -366,18 +374,12 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
 #pragma unroll
       for (int e = 0; e < 2; ++e) {  // dims 32 b + 16 e + 0..15
         const int dt = 2 * b + e;
-        const uint4 c = vc(Q8 ? dt : b);
+        const uint4 c = codes[(NK + (Q8 ? dt : b)) % kDepth];
         h8v v0, v1;
         if constexpr (Q8) v0 = Codes8(c.x, c.y), v1 = Codes8(c.z, c.w);
         else if (e == 0) v0 = NibblesLo8(c.x, c.y), v1 = NibblesLo8(c.z, c.w);
         else v0 = NibblesHi8(c.x, c.y), v1 = NibblesHi8(c.z, c.w);
-        if constexpr (Q8) {
-          if constexpr (kOneSet) load_k(pgn, dt);
-          else load_v(pgn, dt);
-        } else if (e == 1) {
-          if constexpr (kOneSet) load_k(pgn, b);
-          else load_v(pgn, b);
-        }
+        if (Q8 || e == 1) load(NK + (Q8 ? dt : b) + kDepth);
         v0 *= s0, v1 *= s1;
 #pragma unroll
         for (int i = 0; i < RB; ++i) o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pv[i][0], o[i][dt], 0, 0, 0);
@@ -458,12 +460,57 @@ __device__ __forceinline__ void MergeWaves(const SharedArgs& a, SharedLds<D, RB>
   }
 }
 
+// A piece of a prefix against a block of ROWS of its group's rows, by workgroup. Those that read the same keys (the row
+// blocks of a piece) run on one XCD, side by side.
+struct PrefixPiece {
+  int group, h, piece, first, row0, n_rows, tile0, tile1;  // group -1: nothing; n_rows: rows from row0 on
+  __device__ __forceinline__ size_t Row(const SharedArgs& a, int r) const {  // row r of the block among all (sequence, query head) rows
+    const int G = a.g.group(), rr = row0 + min(r, n_rows - 1);
+    return (size_t(first) + rr / G) * a.g.n_q + size_t(h) * G + rr % G;
+  }
+};
+template <int ROWS>
+__device__ __forceinline__ PrefixPiece FindPiece(const SharedArgs& a) {
+  const int G = a.g.group(), H = a.g.n_kv, lane = threadIdx.x % 64;
+  const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
+  const int pair = xcd + 8 * (local / a.max_blocks), block = local % a.max_blocks;
+  PrefixPiece p{-1, pair % H, pair / H, 0, 0, 0, 0, 0};
+  if (pair >= H * a.n_split) return p;
+  int tiles = 0;
+  for (int j0 = 0, before = 0; j0 < a.n_groups; j0 += 64) {  // lane = group: which one row block `block` lies in
+    const int j = min(j0 + lane, a.n_groups - 1);
+    const int first = GroupFirst(a, j), rows = j0 + lane < a.n_groups ? max(GroupFirst(a, j + 1) - first, 0) * G : 0;
+    const int shared = GroupShared(a, j), n = (rows + ROWS - 1) / ROWS;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += v;
+    }
+    const unsigned long long mine = __ballot(before + incl > block && before + incl - n <= block);
+    if (mine != 0) {
+      const int at = __builtin_ctzll(mine);
+      auto its = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+      p.group = j0 + at, p.row0 = (block - before - its(incl - n)) * ROWS;
+      p.first = its(first), p.n_rows = its(rows) - p.row0, tiles = its(shared) / kTile;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  if (p.group < 0) return p;
+  const int per = PerPiece(tiles, a.n_split);
+  p.tile0 = p.piece * per, p.tile1 = min(p.tile0 + per, tiles);
+  if (p.tile0 >= p.tile1) p.group = -1;
+  return p;
+}
+
 template <int FMT, int D, int PT, int RB>
-__global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs a) {
+__global__ __launch_bounds__(64 * kSharedWaves, RB * D <= 256 ? 2 : 1) void SharedPart(const SharedArgs a) {
   constexpr int ROWS = 16 * RB;
+  constexpr bool TWO = RB * D <= 256;  // workgroups a CU
   const Geom g = a.g;
   const int G = g.group(), H = g.n_kv;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   __shared__ __align__(16) SharedLds<D, RB> lds;
 
   if (static_cast<int>(blockIdx.x) >= a.prefix_groups) {  // ---- a piece of a tail: the query heads of one kv head of a sequence
@@ -479,54 +526,23 @@ __global__ __launch_bounds__(64 * kSharedWaves) void SharedPart(const SharedArgs
     queries.Request(a.q, a.q_dtype, [&](int r) { return row0 + min(r, G - 1); });
     float m[1], l[1];
     f4v o[1][D / 16];
-    StreamKeys<FMT, D, PT, 1>(a, a.table + int64_t(s) * a.stride, k.prefix, h, tile0 + wave, kSharedWaves, tile1, k.tail, queries,
+    StreamKeys<FMT, D, PT, 1, TWO>(a, a.table + int64_t(s) * a.stride, k.prefix, h, tile0 + wave, kSharedWaves, tile1, k.tail, queries,
                               lds1.scales[wave], m, l, o);
     MergeWaves<D, 1>(a, lds1, m, l, o, G, [&](int r) { return row0 + r; }, a.n_split + piece);
     return;
   }
-  // ---- a piece of a prefix against a block of its group's rows. Workgroups that read the same keys (the row blocks of a
-  // piece) run on one XCD, side by side.
-  const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
-  const int pair = xcd + 8 * (local / a.max_blocks), block = local % a.max_blocks;
-  if (pair >= H * a.n_split) return;
-  const int h = pair % H, piece = pair / H;
-  int group = -1, row0 = 0;
-  for (int j0 = 0, before = 0; j0 < a.n_groups; j0 += 64) {  // lane = group: which one row block `block` lies in
-    const int j = j0 + lane;
-    const int n = j < a.n_groups ? (max(GroupFirst(a, j + 1) - GroupFirst(a, j), 0) * G + ROWS - 1) / ROWS : 0;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += v;
-    }
-    const unsigned long long mine = __ballot(before + incl > block && before + incl - n <= block);
-    if (mine != 0) {
-      const int at = __builtin_ctzll(mine);
-      group = j0 + at, row0 = (block - before - __shfl(incl - n, at, 64)) * ROWS;
-      break;
-    }
-    before += __shfl(incl, 63, 64);
-  }
-  group = __builtin_amdgcn_readfirstlane(group), row0 = __builtin_amdgcn_readfirstlane(row0);
-  if (group < 0) return;
-  const int first = GroupFirst(a, group), n_rows = (GroupFirst(a, group + 1) - first) * G;
-  const int shared = GroupShared(a, group), tiles = shared / kTile, per = PerPiece(tiles, a.n_split);
-  const int tile0 = piece * per, tile1 = min(tile0 + per, tiles);
-  if (tile0 >= tile1) return;
-  auto row_of = [&](int r) -> size_t {  // row r of the block: its place among all (sequence, query head) rows
-    const int rr = min(row0 + r, n_rows - 1);
-    return (size_t(first) + rr / G) * g.n_q + size_t(h) * G + rr % G;
-  };
+  const PrefixPiece pp = FindPiece<ROWS>(a);
+  if (pp.group < 0) return;
+  auto row_of = [&](int r) -> size_t { return pp.Row(a, r); };
   QueryRows<D, RB> queries;
   queries.lds = lds.q;
   queries.Request(a.q, a.q_dtype, row_of);
   float m[RB], l[RB];
   f4v o[RB][D / 16];
-  StreamKeys<FMT, D, PT, RB>(a, a.table + int64_t(first) * a.stride, 0, h, tile0 + wave, kSharedWaves, tile1, shared, queries,
-                             lds.scales[wave], m, l, o);
+  StreamKeys<FMT, D, PT, RB, TWO>(a, a.table + int64_t(pp.first) * a.stride, 0, pp.h, pp.tile0 + wave, kSharedWaves, pp.tile1,
+                             pp.tile1 * kTile, queries, lds.scales[wave], m, l, o);
   // (rows of sequences shorter than the prefix leave partials that nobody reads)
-  MergeWaves<D, RB>(a, lds, m, l, o, n_rows - row0, row_of, piece);
+  MergeWaves<D, RB>(a, lds, m, l, o, pp.n_rows, row_of, pp.piece);
 }
 
 // One workgroup per (query head, sequence): the prefix's partials and the tail's, weighed by 2^(m - M) and 1 / l. A group of
@@ -593,16 +609,21 @@ SharedPlan MakeSharedPlan(const Geom& m, int32_t n_seqs, int32_t n_groups, int32
   SharedPlan p;
   const int64_t rows = int64_t(n_seqs) * m.group(), per_group = (rows + n_groups - 1) / n_groups;
   auto blocks = [&](int rb) { return (per_group + 16 * rb - 1) / (16 * rb); };
-  // A tile costs a wave about 4000 cycles of decoding and 1500 for each block of 16 rows, whether or not the rows exist.
-  p.row_blocks = 1;
-  for (int rb = 2; rb <= 3; ++rb)
-    if (blocks(rb) * (8 + 3 * rb) < blocks(p.row_blocks) * (8 + 3 * p.row_blocks)) p.row_blocks = rb;
-  p.max_blocks = static_cast<int32_t>(n_groups == 1 ? blocks(p.row_blocks) : rows / (16 * p.row_blocks) + n_groups);
-  // One workgroup per CU and round. A prefix is cut so that the row blocks of an average group fill one round, a tail into
-  // pieces of at most sixteen tiles (four a wave), and finer while that leaves CUs idle; a piece has a tile for every wave.
   const int64_t cus = ComputeUnits(), pre_tiles = max_shared / kTile, tail_tiles = (int64_t(max_tail) + kTile - 1) / kTile;
+  // One row block a wave, or as many as registers allow (three of 128 dims would, but two leave a CU two workgroups:
+  // 256 rows of an 8K prefix 41 us against 44). Four tiles cost a CU 1.1 us with one, 1.6 us with two, 1.25 us with three,
+  // whose one workgroup a CU also takes 14 us more to begin and to end. (32K keys x 12 rows of 256 dims: 23 us with one, 37
+  // with three; 32K x 384 rows: 223 and 107.)
+  const int most = m.hd == 128 ? 2 : 3;
+  const double work = double(n_groups) * m.n_kv * pre_tiles / cus;
+  p.row_blocks = work * blocks(most) * (most == 2 ? 1.6 : 1.25) + (most == 2 ? 0.0 : 14.0) < work * blocks(1) * 1.1 ? most : 1;
+  p.max_blocks = static_cast<int32_t>(n_groups == 1 ? blocks(p.row_blocks) : rows / (16 * p.row_blocks) + n_groups);
+  // A prefix is cut so that the row blocks of an average group give every CU a workgroup, or two if its registers hold them
+  // and each still has four tiles a wave (256 rows x 32K keys of 128 dims: 95 us, with one 117; 64 rows x 8K: 24 and 20). A
+  // tail is cut into pieces of at most sixteen tiles, and finer while that leaves CUs idle; a piece has a tile for every wave.
   const int64_t per_piece = std::max<int64_t>(1, std::min<int64_t>(int64_t(n_groups) * blocks(p.row_blocks), p.max_blocks)) * m.n_kv;
-  p.n_split = static_cast<int32_t>(std::max<int64_t>(1, std::min((cus + per_piece / 2) / per_piece, (pre_tiles + 3) / 4)));
+  const bool two = p.row_blocks * m.hd <= 256 && 2 * cus / per_piece * 4 * 4 <= pre_tiles;
+  p.n_split = static_cast<int32_t>(std::max<int64_t>(1, std::min((two ? 2 * cus : cus) / per_piece, (pre_tiles + 3) / 4)));
   if (pre_tiles == 0) p.n_split = 0;
   const int64_t tails = int64_t(n_seqs) * m.n_kv;
   p.tail_split = static_cast<int32_t>(std::max<int64_t>(1, std::min(std::max((cus + tails - 1) / tails, (tail_tiles + 15) / 16), (tail_tiles + 3) / 4)));
@@ -616,11 +637,19 @@ SharedPlan MakeSharedPlan(const Geom& m, int32_t n_seqs, int32_t n_groups, int32
 }
 
 template <int FMT, int D, int PT>
-void LaunchShared(const SharedArgs& a, int row_blocks, dim3 grid, hipStream_t st) {
+void LaunchShared(const SharedArgs& all, int row_blocks, dim3 grid, hipStream_t st) {
+  constexpr int MOST = D == 128 ? 2 : 3;
   const dim3 block(64 * kSharedWaves);
-  if (row_blocks == 3) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 3>), grid, block, 0, st, a);
-  else if (row_blocks == 2) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 2>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((SharedPart<FMT, D, PT, 1>), grid, block, 0, st, a);
+  SharedArgs a = all;
+  // Tails that fill the chip twice have a launch of their own, where a CU takes two workgroups of them (64 of 1500 keys
+  // beside 32K shared ones: 136 us, with the prefixes 146).
+  if (row_blocks * D > 256 && grid.x - a.prefix_groups >= 2u * ComputeUnits()) {
+    a.prefix_groups = 0;
+    hipLaunchKernelGGL((SharedPart<FMT, D, PT, 1>), dim3(grid.x - all.prefix_groups), block, 0, st, a);
+    grid.x = a.prefix_groups = all.prefix_groups;
+  }
+  if (row_blocks == 1) hipLaunchKernelGGL((SharedPart<FMT, D, PT, 1>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((SharedPart<FMT, D, PT, MOST>), grid, block, 0, st, a);
 }
 template <int FMT>
 void LaunchSharedFormat(const SharedArgs& a, int row_blocks, dim3 grid, hipStream_t st) {
