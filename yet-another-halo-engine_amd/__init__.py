@@ -756,11 +756,19 @@ class Rotary:
 
 def _rows(t, what):
     """A [n_seqs][n_new][heads][D] tensor, each head's values contiguous, as yahkv_rows."""
-    if t.dim() != 4 or t.dtype not in _DTYPES or t.numel() == 0 or t.stride(3) != 1:
+    code, shape, stride = _DTYPES.get(t.dtype), t.shape, t.stride()
+    if code is None or len(shape) != 4 or stride[3] != 1 or t.numel() == 0:
         _refuse(f"{what}: rows [n_seqs][n_new][heads][D] with contiguous heads are expected")
-    n, new, heads, _ = t.shape
-    a, b, c, _ = t.stride()  # (the stride of a dimension of one says nothing)
-    return Rows(t.data_ptr(), _DTYPES[t.dtype], heads, a if n > 1 else 0, b if new > 1 else 0, c if heads > 1 else 0)
+    n, new, heads, _ = shape
+    a, b, c, _ = stride  # (the stride of a dimension of one says nothing)
+    return Rows(t.data_ptr(), code, heads, a if n > 1 else 0, b if new > 1 else 0, c if heads > 1 else 0)
+
+
+def _new_rows(shape, dtype, device):
+    """A new contiguous tensor of the (checked) rows' shape, and it as yahkv_rows."""
+    t = torch.empty(shape, dtype=dtype, device=device)
+    _, new, heads, d = shape
+    return t, Rows(t.data_ptr(), _DTYPES[dtype], heads, new * heads * d, heads * d, d)
 
 
 def _ref(s):
@@ -775,24 +783,34 @@ def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_d
     if first is None or first.dim() != 4:
         _refuse("rotary_rows: q or k [n_seqs][n_new][heads][D]")
     n_seqs, n_new, _, d = first.shape
-    _ints(positions, (n_seqs, n_new), first.device, "positions")
+    dev = first.device
+    _ints(positions, (n_seqs, n_new), dev, "positions")
     rotary.check_head(d)
-    _need(rotary.turns.device == first.device, "rotary_rows: the frequency table is on another device")
-    args, outs = [], []
+    if rotary.turns.device != dev:
+        _refuse("rotary_rows: the frequency table is on another device")
+    refs, outs = [], []
     for x, out in ((q, q_out), (k, k_out)):
         if x is None:
             _need(out is None, "rotary_rows: an output without its rows")
-            args += [None, None]
+            refs += (None, None)
             outs.append(None)
             continue
-        _need(tuple(x.shape[:2]) == (n_seqs, n_new) and x.shape[3] == d and x.device == first.device, "rotary_rows: q and k differ")
+        shape, dtype = x.shape, out_dtype or x.dtype
+        if x is not first and (shape[:2] != (n_seqs, n_new) or shape[3:] != (d,) or x.device != dev):
+            _refuse("rotary_rows: q and k differ")
+        src = _rows(x, "rotary_rows")
         if out is None:
-            out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
-        _need(out.shape == x.shape and out.device == x.device, "rotary_rows: out has the rows' shape")
-        args += [_rows(x, "rotary_rows"), _rows(out, "rotary_rows")]
+            if dtype not in _DTYPES:
+                _refuse(f"rotary_rows: out_dtype {dtype}")
+            out, dst = _new_rows(shape, dtype, dev)
+        else:
+            if out.shape != shape or out.device != dev:
+                _refuse("rotary_rows: out has the rows' shape")
+            dst = _rows(out, "rotary_rows")
+        refs += (C.byref(src), C.byref(dst))
         outs.append(out)
-    _run_on(first.device, lambda st: lib.yahkv_rotary_apply(
-        C.byref(rotary.struct), d, _dp(positions), n_seqs, n_new, *map(_ref, args), st), "rotary_apply")
+    _run_on(dev, lambda st: lib.yahkv_rotary_apply(C.byref(rotary.struct), d, positions.data_ptr(), n_seqs, n_new, *refs, st),
+            "rotary_apply")
     return tuple(outs)
 
 
@@ -818,16 +836,19 @@ def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None,
     if q is not None:
         if q.shape != (n_seqs, n_new, g.n_q_heads, g.head_dim) or q.dtype != k.dtype or q.device != dev:
             _refuse(f"rotary_append: q [n_seqs][n_new][{g.n_q_heads}][{g.head_dim}] of k's type is expected")
+        qs = _rows(q, "q")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q_out_dtype or torch.float32, device=dev)
-        _need(q_out.shape == q.shape and q_out.device == dev, "rotary_append: q_out has q's shape")
-        qs, qd = _rows(q, "q"), _rows(q_out, "q_out")
+            _need(q_out_dtype is None or q_out_dtype in _DTYPES, "rotary_append: q_out_dtype")
+            q_out, qd = _new_rows(q.shape, q_out_dtype or torch.float32, dev)
+        else:
+            _need(q_out.shape == q.shape and q_out.device == dev, "rotary_append: q_out has q's shape")
+            qd = _rows(q_out, "q_out")
     _need(q is not None or q_out is None, "rotary_append: q_out without q")
     _need(k_out is None or (k_out.dtype == torch.float32 and k_out.is_contiguous() and k_out.shape == k.shape and
                             k_out.device == dev), "rotary_append: k_out is contiguous f32 of k's shape")
     st, ks, vs = pools.struct(), _rows(k, "k"), _rows(v, "v")
     _run_on(dev, lambda stream: lib.yahkv_rotary_append(
-        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(start_pos), _dp(n_valid), n_seqs, n_new,
+        C.byref(g), C.byref(st), table.data_ptr(), table.shape[1], start_pos.data_ptr(), _dp(n_valid), n_seqs, n_new,
         C.byref(rotary.struct), _dp(positions), C.byref(ks), C.byref(vs), _ref(qs), _ref(qd), _dp(k_out), stream),
         "rotary_append")
     return q_out
@@ -856,9 +877,9 @@ def decode_attend_shared(pools, table, seq_len, group_first, shared_len, max_sha
     workspace = _scratch(workspace, lambda: decode_shared_workspace_bytes(g, n_seqs, n_groups, max_shared_len, max_tail_len), dev)
     st = pools.struct()
     _run_on(dev, lambda stream: lib.yahkv_decode_attend_shared(
-        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(seq_len), n_seqs, _dp(group_first), _dp(shared_len),
-        n_groups, max_shared_len, max_tail_len, _dp(q), _dtype_code(q), scale, _dp(gate), _dp(out), _dtype_code(out),
-        _dp(workspace), workspace.numel(), stream), "decode_attend_shared")
+        C.byref(g), C.byref(st), table.data_ptr(), table.shape[1], seq_len.data_ptr(), n_seqs, group_first.data_ptr(),
+        shared_len.data_ptr(), n_groups, max_shared_len, max_tail_len, q.data_ptr(), _DTYPES[q.dtype], scale, _dp(gate),
+        out.data_ptr(), _DTYPES[out.dtype], workspace.data_ptr(), workspace.numel(), stream), "decode_attend_shared")
     return out
 
 
@@ -889,9 +910,9 @@ def decode_attend_weights(pools, table, seq_len, max_seq_len, q, scale, weights_
     workspace = _scratch(workspace, lambda: decode_weights_workspace_bytes(g, n_seqs, max_seq_len), dev)
     st = pools.struct()
     _run_on(dev, lambda stream: lib.yahkv_decode_attend_weights(
-        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(seq_len), n_seqs, max_seq_len, _dp(q), _dtype_code(q),
-        scale, _dp(gate), _dp(out), _dtype_code(out), _dp(weights_in), _dp(weights_out), weights_out.shape[2], decay,
-        _dp(workspace), workspace.numel(), stream), "decode_attend_weights")
+        C.byref(g), C.byref(st), table.data_ptr(), table.shape[1], seq_len.data_ptr(), n_seqs, max_seq_len, q.data_ptr(),
+        _DTYPES[q.dtype], scale, _dp(gate), out.data_ptr(), _DTYPES[out.dtype], _dp(weights_in), weights_out.data_ptr(),
+        weights_out.shape[2], decay, workspace.data_ptr(), workspace.numel(), stream), "decode_attend_weights")
     return out
 
 
@@ -910,8 +931,8 @@ def evict_select(g, seq_len, max_seq_len, weights, budget, sink=0, recent=0, kep
     _ints(kept, (n_seqs, g.n_kv_heads, max(budget, 0)), dev, "kept")
     _ints(n_kept, (n_seqs,), dev, "n_kept")
     _run_on(dev, lambda stream: lib.yahkv_evict_select(
-        C.byref(g), _dp(seq_len), n_seqs, max_seq_len, _dp(weights), weights.shape[2], budget, sink, recent, _dp(kept),
-        _dp(n_kept), stream), "evict_select")
+        C.byref(g), seq_len.data_ptr(), n_seqs, max_seq_len, weights.data_ptr(), weights.shape[2], budget, sink, recent,
+        kept.data_ptr(), n_kept.data_ptr(), stream), "evict_select")
     return kept, n_kept
 
 
@@ -932,8 +953,8 @@ def evict_compact(pools, table, kept, n_kept, dst_table, weights_in=None, weight
         _weight_rows(weights_out, g, n_seqs, budget, dev, "weights_out")
     st = pools.struct()
     _run_on(dev, lambda stream: lib.yahkv_evict_compact(
-        C.byref(g), C.byref(st), _dp(table), table.shape[1], _dp(kept), _dp(n_kept), n_seqs, budget, _dp(dst_table),
-        dst_table.shape[1], _dp(weights_in), 0 if weights_in is None else weights_in.shape[2], _dp(weights_out),
+        C.byref(g), C.byref(st), table.data_ptr(), table.shape[1], kept.data_ptr(), n_kept.data_ptr(), n_seqs, budget,
+        dst_table.data_ptr(), dst_table.shape[1], _dp(weights_in), 0 if weights_in is None else weights_in.shape[2], _dp(weights_out),
         0 if weights_out is None else weights_out.shape[2], stream), "evict_compact")
 
 
