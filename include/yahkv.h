@@ -415,7 +415,8 @@ typedef struct yahkv_rotary {
   const float* k_weight;
 } yahkv_rotary;
 /* Rows of head_dim values, [n_seqs][n_new][n_heads] of them at element strides of their own (slices of a fused projection,
- * head-major tensors). data is 16-byte aligned and every stride a multiple of 16 bytes. */
+ * head-major tensors). data is 16-byte aligned and every stride a multiple of 16 bytes; no two rows of a destination overlap
+ * (strides of 0 there are refused, source rows may repeat). */
 typedef struct yahkv_rows {
   void* data;
   int32_t dtype;    /* yahkv_dtype */
@@ -467,7 +468,7 @@ int yahkv_decode_attend_shared(const yahkv_geometry* g, const yahkv_pools* pools
  * Decode attention that also leaves what each key weighed: for t < seq_len[s]
  *   weights_out[s][h][t] = decay * weights_in[s][h][t] + sum over kv head h's query heads of softmax weight t
  * with f32 rows [n_seqs][n_kv_heads][weights_stride]; weights_in may be NULL (zeros) or weights_out itself; entries at or
- * past the length are not touched. out is of out_dtype (F32, F16 or BF16); other arguments as yahkv_decode_attend. The weights
+ * past the length are not touched (a new token's entry is read in its first step: clear the rows before a sequence begins). out is of out_dtype (F32, F16 or BF16); other arguments as yahkv_decode_attend. The weights
  * are f32 throughout (scores from the exact codes), whatever out_dtype; lengths above max_seq_len or above weights_stride
  * are clamped, and max_seq_len may not exceed weights_stride. Three dispatches. */
 size_t yahkv_decode_weights_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t max_seq_len);
@@ -488,8 +489,8 @@ int yahkv_evict_select(const yahkv_geometry* g, const int32_t* seq_len, int32_t 
  * sequence s's new pages dst_table[s][0 .. ceil(budget / PT)), and weights_in[s][h][kept[s][h][i]] to weights_out[s][h][i]
  * (both NULL: no weights). Slots at or past n_kept[s] are left as they are. New pages must not be pages that any source
  * row of this call names: sources may be shared with other sequences, so nothing is moved in place; take fresh pages from the
- * allocator, upload their row in place of the old one, and free the old pages behind the call in stream order. Afterwards the sequence
- * is n_kept[s] tokens long, and its next token goes to slot n_kept[s] at its own position (yahkv_rotary_append). Kept
+ * allocator, upload their row in place of the old one, and free the old pages behind the call in stream order. weights_out may
+ * not overlap weights_in. Afterwards the sequence is n_kept[s] tokens long, and its next token goes to slot n_kept[s] at its own position (yahkv_rotary_append). Kept
  * positions are clamped to the table, pages to the pool. */
 int yahkv_evict_compact(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
                         int32_t page_table_stride, const int32_t* kept, const int32_t* n_kept, int32_t n_seqs,

@@ -115,6 +115,19 @@ def test_strided_in_place_and_alone(yahkv, torch_gpu, n, new):
     assert torch.equal(x[:, :, :8], qo) and torch.equal(x[:, :, 8:10], ko) and torch.equal(x[:, :, 10:], before[:, :, 10:])
 
 
+def test_repeated_source_rows(yahkv, torch_gpu):
+    """One row for all heads and all sequences (strides of 0) on the way in; on the way out it is refused."""
+    torch = torch_gpu
+    x = torch.randn(1, 5, 1, 128, device="cuda").half()
+    r = make(yahkv, 64, "half", "none")
+    pos = torch.arange(15, dtype=torch.int32, device="cuda").view(3, 5)
+    got, _ = yahkv.rotary_rows(r, pos, x.expand(3, 5, 4, 128))
+    want, _ = yahkv.rotary_rows(r, pos, x.expand(3, 5, 4, 128).contiguous())
+    assert torch.equal(got, want)
+    with pytest.raises(yahkv.YahkvError):
+        yahkv.rotary_rows(r, pos, x.expand(3, 5, 4, 128), q_out=torch.empty_like(x).expand(3, 5, 4, 128))
+
+
 def test_untouched_dims_pass_through_infinities(yahkv, torch_gpu):
     """Dims that are not rotated are the source's bits, NaN and infinities among them; a pair with one is not finite."""
     torch = torch_gpu

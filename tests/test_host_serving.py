@@ -113,6 +113,16 @@ def test_rotary_apply_refusals(yahkv):
     assert apply(yahkv, n=1 << 20, new=1 << 20) == SHAPE
 
 
+def test_destination_rows_at_one_address_are_refused(yahkv):
+    for kw in (dict(seq_stride=0), dict(token_stride=0), dict(head_stride=0)):
+        assert apply(yahkv, n=2, new=2, qd=rows(yahkv, 8, **kw)) == ARG, kw
+        assert apply(yahkv, n=2, new=2, kd=rows(yahkv, 2, **kw)) == ARG, kw
+    g = yahkv.geometry(8, 8, 2, 128, 16, 4)
+    k, v, q, out = rows(yahkv, 2), rows(yahkv, 2), rows(yahkv, 8), rows(yahkv, 8, token_stride=0)
+    assert yahkv.lib.yahkv_rotary_append(C.byref(g), C.byref(pools(yahkv, g)), P, 4, P, None, 1, 9, C.byref(rotary(yahkv)), None,
+                                         C.byref(k), C.byref(v), C.byref(q), C.byref(out), None, None) == ARG
+
+
 def pools(yahkv, g, **kw):
     b = yahkv.pool_bytes(g)
     f = dict(kq=P, ks=P, vq=P, vs=P, kq_bytes=b["kq"], ks_bytes=b["ks"], vq_bytes=b["vq"], vs_bytes=b["vs"])

@@ -621,7 +621,7 @@ extern "C" int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* p
   if ((q_src == nullptr) != (q_dst == nullptr) || !Aligned16(k_out)) return YAHKV_ERR_ARG;
   if (q_src != nullptr) {
     if (const int st = CheckRows(q_src, &a.q_rows)) return st;
-    if (const int st = CheckRows(q_dst, &a.q_out_rows)) return st;
+    if (const int st = CheckRowsOut(q_dst, n_seqs, n_new, &a.q_out_rows)) return st;
     if (q_src->n_heads != g->n_q_heads || q_dst->n_heads != g->n_q_heads || q_src->dtype != k->dtype) return YAHKV_ERR_ARG;
     a.q_src = q_src->data, a.q_out = q_dst->data, a.q_out_dtype = q_dst->dtype;
   }

@@ -193,12 +193,12 @@ extern "C" int yahkv_rotary_apply(const yahkv_rotary* rotary, int32_t head_dim, 
   if (q_src == nullptr && k_src == nullptr) return YAHKV_ERR_ARG;
   if (q_src != nullptr) {
     if (const int st = CheckRows(q_src, &a.qs)) return st;
-    if (const int st = CheckRows(q_dst, &a.qd)) return st;
+    if (const int st = CheckRowsOut(q_dst, n_seqs, n_new, &a.qd)) return st;
     if (a.qs.n_heads != a.qd.n_heads) return YAHKV_ERR_ARG;
   }
   if (k_src != nullptr) {
     if (const int st = CheckRows(k_src, &a.ks)) return st;
-    if (const int st = CheckRows(k_dst, &a.kd)) return st;
+    if (const int st = CheckRowsOut(k_dst, n_seqs, n_new, &a.kd)) return st;
     if (a.ks.n_heads != a.kd.n_heads || (q_src != nullptr && a.ks.dtype != a.qs.dtype)) return YAHKV_ERR_ARG;
   }
   const int64_t tokens = int64_t(n_seqs) * n_new, rows = int64_t(a.qs.n_heads) + a.ks.n_heads;

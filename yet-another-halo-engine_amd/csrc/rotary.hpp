@@ -63,6 +63,13 @@ inline int CheckRows(const yahkv_rows* r, RowsArgs* a) {
   return YAHKV_OK;
 }
 
+// Destination rows: two tokens or heads at one address would be written in any order.
+inline int CheckRowsOut(const yahkv_rows* r, int32_t n_seqs, int32_t n_new, RowsArgs* a) {
+  if (const int st = CheckRows(r, a)) return st;
+  if ((n_seqs > 1 && a->seq == 0) || (n_new > 1 && a->token == 0) || (a->n_heads > 1 && a->head == 0)) return YAHKV_ERR_ARG;
+  return YAHKV_OK;
+}
+
 // The rows kernel (rotary.hip): q and / or k rows (n_heads 0: none) of n_seqs x n_new tokens, turned by positions[s][t] or,
 // where that is null, by start_pos[s] + t; rows at or past n_valid[s] (null: n_new) are left alone. Arguments are checked.
 int LaunchRotaryRows(const RotaryArgs& r, int32_t head_dim, const int32_t* positions, const int32_t* start_pos,

@@ -86,8 +86,8 @@ __device__ __forceinline__ Keys KeysOf(const SharedArgs& a, int s) {
   const int shared = j < 0 ? 0 : GroupShared(a, j), prefix = len < shared ? 0 : shared;
   return Keys{prefix, min(len - prefix, a.max_tail)};
 }
-// `tiles` cut into at most n pieces: tiles per piece
-__device__ __forceinline__ int PerPiece(int tiles, int n) { return max((tiles + n - 1) / n, 1); }
+// `tiles` cut into at most n pieces (0 where the host allows no prefix): tiles per piece
+__device__ __forceinline__ int PerPiece(int tiles, int n) { return max((tiles + n - 1) / max(n, 1), 1); }
 
 // Maximum and sum over the four lane groups of a wave (lanes n, n + 16, n + 32, n + 48), in every lane.
 template <typename Op>
