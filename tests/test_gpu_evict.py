@@ -195,6 +195,46 @@ def test_compact(yahkv, torch_gpu, fmt, n_kv, hd, pt, budget):
     assert np.array_equal(w_out.cpu().numpy(), want_w)
 
 
+def test_choice_and_move_from_a_graph(yahkv, torch_gpu):
+    torch = torch_gpu
+    rng = np.random.default_rng(1)
+    lens, budget, pt = [400, 33, 200], 100, 32
+    g = yahkv.geometry(8, 8, 2, 128, pt, 64)
+    b = yahkv.pool_bytes(g)
+    dev, ref = yahkv.DevicePools(g), yahkv.DevicePools(g)
+    arrays = {k: rng.integers(0, 256, b[k], dtype=np.uint8) for k in b}
+    perm = rng.permutation(64).astype(np.int32)
+    t = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    table, dst = t(perm[:39].reshape(3, 13)), t(perm[39:51].reshape(3, 4))
+    seq_len, w = t(np.array(lens, np.int32)), torch.rand(3, 2, 400, device="cuda")
+    kept, n_kept = torch.zeros(3, 2, budget, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    w_out = torch.zeros(3, 2, budget, device="cuda")
+
+    def run(pools, kept, n_kept, w_out):
+        yahkv.evict_select(g, seq_len, 400, w, budget, 4, 16, kept=kept, n_kept=n_kept)
+        yahkv.evict_compact(pools, table, kept, n_kept, dst, w, w_out)
+
+    dev.load(arrays)
+    run(dev, kept, n_kept, w_out)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            run(dev, kept, n_kept, w_out)
+    for i in range(3):
+        w.copy_(torch.rand(3, 2, 400, device="cuda"))
+        seq_len.copy_(t(np.array([lens[(i + j) % 3] for j in range(3)], np.int32)))
+        want = [torch.zeros_like(x) for x in (kept, n_kept, w_out)]
+        dev.load(arrays), ref.load(arrays)
+        run(ref, *want)
+        w_out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip((kept, n_kept, w_out, dev.kq, dev.ks, dev.vq, dev.vs), (*want, ref.kq, ref.ks, ref.vq, ref.vs)):
+            assert torch.equal(x, y), i
+
+
 def test_compact_clamps_what_it_reads(yahkv, torch_gpu):
     """Kept positions past the table and page numbers past the pool are cut to them, a count past the budget to the budget."""
     torch = torch_gpu
