@@ -794,7 +794,8 @@ void DattnPart(const DecodeArgs a) {
 // registers the K codes leave. Its result for the pair goes to the wave's LDS slot (V does not pass through LDS
 // here), where a second tile of the same pair joins it and where the workgroup's merge finds it, so nothing but the
 // tile in hand occupies registers. Wave w takes tiles w, w + 8, ... of the chunk: the same sums in the same order on
-// every run.
+// every run. WEIGH as in DattnPart (one 32K sequence: 22.6 us, DattnPart 24.6).
+template <bool WEIGH>
 __global__ __launch_bounds__(64 * kWavesPerGroup) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void DattnPartWhole(const DecodeArgs a) {
   constexpr int D = 256, PT = kTile, NB = D / 32, NT = D / 16, NVB = NT / 2, QE = NB * 32 / 64;
@@ -867,6 +868,7 @@ void DattnPartWhole(const DecodeArgs a) {
     vsr = StreamLoad(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pools.vs) + ph * (NB * PT * 2) +
                                                     (b * PT + 8 * chunk) * 2));
   };
+  auto kcodes = [](uint32_t w0, uint32_t w1) -> h8v { return WEIGH ? Codes8(w0, w1) : RawCodes8(w0, w1); };
   // scores of the 32 keys of half tt against all heads: two blocks (two accumulator chains) at a time
   auto scores = [&](int tt) {
 #pragma unroll
@@ -881,10 +883,10 @@ void DattnPartWhole(const DecodeArgs a) {
       const float4 k1 = *reinterpret_cast<const float4*>(&lcorr[b + 1][4 * half]);
       const float kc0[4] = {k0.x, k0.y, k0.z, k0.w}, kc1[4] = {k1.x, k1.y, k1.z, k1.w};
       f16v c0 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}, c1 = c0;
-      c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qa0, RawCodes8(kb[tt][b][0], kb[tt][b][1]), c0, 0, 0, 0);
-      c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qb0, RawCodes8(kb[tt][b + 1][0], kb[tt][b + 1][1]), c1, 0, 0, 0);
-      c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qa1, RawCodes8(kb[tt][b][2], kb[tt][b][3]), c0, 0, 0, 0);
-      c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qb1, RawCodes8(kb[tt][b + 1][2], kb[tt][b + 1][3]), c1, 0, 0, 0);
+      c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qa0, kcodes(kb[tt][b][0], kb[tt][b][1]), c0, 0, 0, 0);
+      c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qb0, kcodes(kb[tt][b + 1][0], kb[tt][b + 1][1]), c1, 0, 0, 0);
+      c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qa1, kcodes(kb[tt][b][2], kb[tt][b][3]), c0, 0, 0, 0);
+      c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(qb1, kcodes(kb[tt][b + 1][2], kb[tt][b + 1][3]), c1, 0, 0, 0);
       const uint32_t w = b < 2 ? ksc[tt].x : b < 4 ? ksc[tt].y : b < 6 ? ksc[tt].z : ksc[tt].w;  // scales of blocks b, b + 1
       const float d0 = WidenF16(static_cast<uint16_t>(w & 0xFFFF)) * qk_scale;
       const float d1 = WidenF16(static_cast<uint16_t>(w >> 16)) * qk_scale;
@@ -961,7 +963,7 @@ void DattnPartWhole(const DecodeArgs a) {
         float t = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) t += static_cast<float>(qv[k]);
-        t *= 1152.0f;
+        t *= WEIGH ? 0.0f : 1152.0f;
         t += __shfl_xor(t, 8, 64);
         t += __shfl_xor(t, 16, 64);
         if (lane % 32 < 8) lcorr[i / 32][i % 8] = t;
@@ -978,7 +980,14 @@ void DattnPartWhole(const DecodeArgs a) {
     for (int tt = 0; tt < 2; ++tt) {
       const bool valid = tile * kTile + 32 * tt + n32 < cur.len;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[tt][r] = valid ? sc[tt][r] : kNegMax;
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (WEIGH) {
+          const int row = 4 * half + r;
+          if (valid && row < G)
+            a.scores[(size_t(cur.s) * g.n_q + size_t(cur.h) * G + row) * a.score_stride + tile * kTile + 32 * tt + n32] = sc[tt][r];
+        }
+        sc[tt][r] = valid ? sc[tt][r] : kNegMax;
+      }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -1300,7 +1309,8 @@ int LaunchPart(const DecodeArgs& a, hipStream_t st) {
   const Geom& m = a.g;
   const dim3 grid(static_cast<unsigned>(a.n_chunks));
   if (a.whole_tiles) {  // (Prepare sets it for q8_0, head_dim 256, 64-token pages and a small batch only)
-    hipLaunchKernelGGL(DattnPartWhole, grid, dim3(64 * kWavesPerGroup), 0, st, a);
+    if (a.scores != nullptr) hipLaunchKernelGGL(DattnPartWhole<true>, grid, dim3(64 * kWavesPerGroup), 0, st, a);
+    else hipLaunchKernelGGL(DattnPartWhole<false>, grid, dim3(64 * kWavesPerGroup), 0, st, a);
     return LaunchStatus();
   }
 #define YAHKV_LAUNCH_PART(FF, DD, PP)                                                                          \
@@ -1493,14 +1503,14 @@ extern "C" int yahkv_decode_attend(const yahkv_geometry* g, const yahkv_pools* p
 }
 
 namespace {
-// The two-dispatch forms (the whole-tile kernel does not weigh). A batch of at most four tiles per wave is cut into chunks of
-// one tile per wave, a pair's change costs nothing, and a workgroup leaves one partial of its last pair (one 32K sequence:
-// merge 17.6 -> 8 us); a larger one leaves a partial per wave.
+// The two-dispatch forms. A batch of at most four tiles per wave is cut into chunks of one tile per wave, a pair's change costs
+// nothing, and a workgroup leaves one partial of its last pair (one 32K sequence: merge 17.6 -> 8 us), by the whole-tile kernel
+// where it applies; a larger one leaves a partial per wave.
 yahkv_decode_options WeighOptions(const Geom& m, int32_t n_seqs, int32_t max_seq_len) {
   const int64_t tiles = (int64_t(max_seq_len) + kTile - 1) / kTile * n_seqs * m.n_kv;
   const bool small = tiles <= int64_t(ComputeUnits()) * kWavesPerGroup * 4;
   yahkv_decode_options o{};
-  o.wg_partials = small ? 1 : 2;
+  o.wg_partials = small ? 3 : 2;
   if (small) o.min_chunk_tiles = kWavesPerGroup, o.pair_cost = -1;
   return o;
 }
