@@ -66,14 +66,16 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
   while ((kSelectThreads << lg_own) < min(len, kSegment)) ++lg_own;
   const int own = 1 << lg_own;
   int loaded = -1;
-  auto load = [&](int seg) {  // (a barrier on either side; nothing if it is there already)
+  auto load_and = [&](int seg, auto also) {  // (a barrier on either side; nothing if it is there already); also(key) for each
     if (seg == loaded) return;
     __syncthreads();
     const int base = seg * kSegment, n = min(len - base, kSegment);
     const float* const from = w + base;
     auto put = [&](int e, float v) {
       const int t = base + e;
-      keys[(e >> lg_own) * (kOwn + 1) + (e & (own - 1))] = t >= len ? 0u : t < lo || t >= hi ? kAlways : WeightKey(v);
+      const uint32_t key = t >= len ? 0u : t < lo || t >= hi ? kAlways : WeightKey(v);
+      keys[(e >> lg_own) * (kOwn + 1) + (e & (own - 1))] = key;
+      also(key);
     };
     const int n4 = (reinterpret_cast<uintptr_t>(from) & 15) == 0 ? n & ~3 : 0;
 #pragma unroll 8
@@ -85,6 +87,7 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
     loaded = seg;
     __syncthreads();
   };
+  auto load = [&](int seg) { load_and(seg, [](uint32_t) {}); };
   auto each = [&](auto f) {  // f(key, its place among this thread's keys of the segment), in order
     for (int j0 = 0; j0 < own; j0 += 8) {
       uint32_t k[8];
@@ -140,12 +143,10 @@ __global__ __launch_bounds__(kSelectThreads) void EvictSelect(const SelectArgs a
   if (any) {  // (the sign bit is never set: eleven bits from bit 30 down)
     if (tid == 0) list_n = 0;
     clear_bins();
-    for (int seg = 0; seg < n_segments; ++seg) {
-      load(seg);
-      each([&](uint32_t key, int) {
+    for (int seg = 0; seg < n_segments; ++seg)  // (counted on their way in)
+      load_and(seg, [&](uint32_t key) {
         if (Weighed(key)) atomicAdd(&bins[key >> 20], 1u);
       });
-    }
     find_digit(20, 2047u);
     const bool listed = found[2] <= static_cast<uint32_t>(kListed);
     const uint32_t top = prefix, top_mask = mask;
