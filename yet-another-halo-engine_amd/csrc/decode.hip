@@ -1269,7 +1269,8 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
 
 // weights_out[s][h][t] = decay * weights_in[s][h][t] + sum over the head's query rows of e^(score - M) / l: a thread per
 // key, the rows' maxima and sums the same for a workgroup. Reads 4 G + 4 and writes 4 bytes a key, a tenth of what the
-// key's K and V rows take.
+// key's K and V rows take (24 ragged sequences of up to 16K, 32 + 8 heads of 128 dims in 4 bits: 9.4 us beside the part
+// kernel's 70, of which leaving the scores takes 3).
 struct WeighArgs {
   const int32_t* seq_len;
   const float* scores;

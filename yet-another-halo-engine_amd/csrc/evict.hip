@@ -8,10 +8,14 @@
 // which go to a list in LDS for the rest. One workgroup does it all, with the row in its LDS; a thread owns consecutive
 // keys, so that the kept positions come out in order from its own count and one scan over the threads. What bounds it is the
 // instructions of the one CU that a row has: loops over lanes' own keys with a few instructions a key, not wave-wide votes.
+// One 32K row a head, cut to 4K: 20.6 us (5 to load and count, 2.4 the list, 2.5 two digits, 5.3 the places and the way out;
+// the rest launch and scans); 32 ragged rows of up to 16K for each of 4 heads: 15.6 us.
 //
 // The move. A workgroup fills one new page of one kv head. K blocks are contiguous pieces of 32 (or 16) bytes; V lies
 // transposed, so that a key is a byte in each of its rows, and any key of a page costs that page's whole V region in lines
-// from memory: kept keys spread over all pages mean that all of V is read, whatever the budget.
+// from memory: kept keys spread over all pages mean that all of V is read, whatever the budget. 32 ragged sequences of up to 16K
+// cut to 2K, 4 heads of 256 dims: 119 us for 442 MB of lines read and 163 MB written, 5.1 TB/s, a large copy's rate on this
+// card (4.85); one of 32K cut to 4K: 15.3 us.
 #include "common.hpp"
 #include "quant.hpp"
 

@@ -546,7 +546,8 @@ __global__ __launch_bounds__(64 * kSharedWaves, RB * D <= 256 ? 2 : 1) void Shar
 }
 
 // One workgroup per (query head, sequence): the prefix's partials and the tail's, weighed by 2^(m - M) and 1 / l. A group of
-// D / 4 lanes takes every n-th partial, four dims a lane; the groups' sums meet in LDS.
+// D / 4 lanes takes every n-th partial, four dims a lane; the groups' sums meet in LDS. (64 x 24 rows of up to ten partials of 256
+// dims: 6.9 us, a round trip behind a round trip; the partials are in the caches.)
 struct MergeArgs {
   SharedArgs s;
   const float* gate;
