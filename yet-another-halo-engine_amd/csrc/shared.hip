@@ -18,6 +18,10 @@
 // A register is asked for again (for the wave's next tile) as soon as its codes are decoded, so a load has about a tile's
 // time to arrive, without a barrier anywhere in the loop. Decoding is packed f16 arithmetic, perm, add, multiply for two
 // values, the product d * code rounded once and saturated at the largest finite f16 (SetSaturation).
+// Roundings to f16 (11 bits): queries given as f32, K, V and the numerators, each once; products and sums are f32. With scores
+// of a standard deviation of two K's costs 3.5e-4 of the output's norm, the numerators' 2.0e-4, V's 1.6e-4 (an f16 output's own
+// is 2.1e-4). Exact K codes with their scales on the sums instead would take 12 multiplications for every 4 saved here with
+// three row blocks, a tenth of the kernel's time.
 //
 // What bounds it: with few rows the reads and a workgroup's beginning and end (12 query rows on 32K keys of 4 x 256 dims: 23
 // us, 71 MB); with three row blocks of 256 dims the vector unit, which issues 1470 instructions of 4 cycles for a tile's 192
