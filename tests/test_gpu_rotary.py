@@ -115,6 +115,20 @@ def test_strided_in_place_and_alone(yahkv, torch_gpu, n, new):
     assert torch.equal(x[:, :, :8], qo) and torch.equal(x[:, :, 8:10], ko) and torch.equal(x[:, :, 10:], before[:, :, 10:])
 
 
+@pytest.mark.parametrize("tokens", [2, 1030])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_many_rows_a_token_in_place(yahkv, torch_gpu, tokens, layout):
+    """More rows than a workgroup has on its way at once, an odd number of them."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    x = torch.randn(1, tokens, 40, 256, generator=gen, device="cuda")
+    pos = torch.randint(-5, 100000, (1, tokens), generator=gen, device="cuda", dtype=torch.int32)
+    r = make(yahkv, 128, layout, "ntk", first_dim=64)
+    want = want_rows(x.double().cpu().numpy(), pos.cpu().numpy(), 128, layout, "ntk", first=64)
+    yahkv.rotary_rows(r, pos, x[:, :, :37], x[:, :, 37:], q_out=x[:, :, :37], k_out=x[:, :, 37:])
+    close(torch, x, want, torch.float32)
+
+
 def test_repeated_source_rows(yahkv, torch_gpu):
     """One row for all heads and all sequences (strides of 0) on the way in; on the way out it is refused."""
     torch = torch_gpu

@@ -6,8 +6,8 @@
 // cosines and sines (they depend on the position and the pair, not on the head) are worked out once into LDS, one pair
 // a thread, and its rows are dealt to groups of lanes, a lane holding two pieces of four dims. In the half layout the
 // pieces are four first and their four second members, in the interleaved layout they are neighbours: either way a lane
-// holds whole pairs, and no value crosses lanes but the sum of squares. 8 x 2048 tokens of 24 + 4 heads of 256 dims, bf16: 88
-// us for 470 MB, 5.3 TB/s; a step of 64 tokens 7.6 us, most of it the way from positions to sines to rows.
+// holds whole pairs, and no value crosses lanes but the sum of squares. 8 x 2048 tokens of 24 + 4 heads of 256 dims, bf16: 87
+// us for 470 MB, 5.4 TB/s; a step of 64 tokens 4.3 us, most of it the way from positions to sines to rows.
 #include <cmath>
 
 #include "common.hpp"
@@ -28,9 +28,12 @@ struct ApplyArgs {
   RowsArgs qs, qd, ks, kd;   // qs.n_heads may be 0
 };
 
-constexpr int kRowThreads = 256, kRowsAtOnce = 4;
+constexpr int kRowThreads = 256;
 
-template <int SRC>
+// AT_ONCE: rows that a lane has on their way. Two for long calls (8 x 2048 tokens of 28 rows of 256 dims 87 us, with one 90, with
+// four 89; 5 x 1037 tokens of 32 rows of 128: 22.7, 23.3, 25.1), one for short ones, which wait for their code (64 tokens:
+// 4.3 us, with two 5.4, with four 7.5).
+template <int SRC, int AT_ONCE>
 __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
   const int token = blockIdx.x, s = token / a.n_new, t = token % a.n_new;
   const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = kRowThreads / lanes;
@@ -53,10 +56,10 @@ __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
     *rows = &r;
     return s * r.seq + t * r.token + (is_q ? row : row - a.qs.n_heads) * r.head;
   };
-  uint4 raw[kRowsAtOnce][2];
+  uint4 raw[AT_ONCE][2];
   auto request = [&](int row0) {
 #pragma unroll
-    for (int j = 0; j < kRowsAtOnce; ++j) {
+    for (int j = 0; j < AT_ONCE; ++j) {
       const RowsArgs* r;
       const int64_t at = place(min(row0 + slots * j, row_end - 1), true, &r);
       raw[j][0] = LoadRaw4(r->data, at + e0, SRC), raw[j][1] = LoadRaw4(r->data, at + e1, SRC);
@@ -77,13 +80,13 @@ __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
   if (turned) c4 = *reinterpret_cast<const float4*>(&cs[4 * lane]), s4 = *reinterpret_cast<const float4*>(&sn[4 * lane]);
   const bool halves = !turned || a.r.layout == YAHKV_ROTARY_HALF;
 
-  for (int row0 = row_first; row0 < row_end; row0 += slots * kRowsAtOnce) {
-    float4 x[kRowsAtOnce], y[kRowsAtOnce];
+  for (int row0 = row_first; row0 < row_end; row0 += slots * AT_ONCE) {
+    float4 x[AT_ONCE], y[AT_ONCE];
 #pragma unroll
-    for (int j = 0; j < kRowsAtOnce; ++j) x[j] = Widen4(raw[j][0], SRC), y[j] = Widen4(raw[j][1], SRC);
-    if (row0 + slots * kRowsAtOnce < row_end) request(row0 + slots * kRowsAtOnce);
+    for (int j = 0; j < AT_ONCE; ++j) x[j] = Widen4(raw[j][0], SRC), y[j] = Widen4(raw[j][1], SRC);
+    if (row0 + slots * AT_ONCE < row_end) request(row0 + slots * AT_ONCE);
 #pragma unroll
-    for (int j = 0; j < kRowsAtOnce; ++j) {
+    for (int j = 0; j < AT_ONCE; ++j) {
       const int row = row0 + slots * j;
       if (row >= row_end) break;
       float4 u = x[j], v = y[j];
@@ -116,6 +119,13 @@ __global__ __launch_bounds__(kRowThreads) void RotaryRows(const ApplyArgs a) {
   }
 }
 
+template <int AT_ONCE>
+void LaunchRows(int32_t src, dim3 grid, hipStream_t st, const ApplyArgs& a) {
+  if (src == YAHKV_F32) hipLaunchKernelGGL((RotaryRows<YAHKV_F32, AT_ONCE>), grid, dim3(kRowThreads), 0, st, a);
+  else if (src == YAHKV_F16) hipLaunchKernelGGL((RotaryRows<YAHKV_F16, AT_ONCE>), grid, dim3(kRowThreads), 0, st, a);
+  else hipLaunchKernelGGL((RotaryRows<YAHKV_BF16, AT_ONCE>), grid, dim3(kRowThreads), 0, st, a);
+}
+
 }  // namespace
 
 int LaunchRotaryRows(const RotaryArgs& r, int32_t head_dim, const int32_t* positions, const int32_t* start_pos,
@@ -129,14 +139,13 @@ int LaunchRotaryRows(const RotaryArgs& r, int32_t head_dim, const int32_t* posit
   while (a.lanes < head_dim / 8) a.lanes *= 2;
   // Few tokens: a token's rows go to several workgroups, each with one round of loads; many: all rows of a token share
   // one workgroup's sines.
-  const int at_once = kRowThreads / a.lanes * kRowsAtOnce;
-  a.rows_per_group = tokens >= 1024 ? a.n_rows : at_once;
+  const bool few = tokens < 1024;
+  a.rows_per_group = few ? kRowThreads / a.lanes : a.n_rows;
   const unsigned groups = static_cast<unsigned>((a.n_rows + a.rows_per_group - 1) / a.rows_per_group);
   const dim3 grid(static_cast<unsigned>(tokens), groups);
   const int32_t src = q_src.n_heads != 0 ? q_src.dtype : k_src.dtype;
-  if (src == YAHKV_F32) hipLaunchKernelGGL(RotaryRows<YAHKV_F32>, grid, dim3(kRowThreads), 0, st, a);
-  else if (src == YAHKV_F16) hipLaunchKernelGGL(RotaryRows<YAHKV_F16>, grid, dim3(kRowThreads), 0, st, a);
-  else hipLaunchKernelGGL(RotaryRows<YAHKV_BF16>, grid, dim3(kRowThreads), 0, st, a);
+  if (few) LaunchRows<1>(src, grid, st, a);
+  else LaunchRows<2>(src, grid, st, a);
   return LaunchStatus();
 }
 
