@@ -244,6 +244,28 @@ def test_append_without_queries_or_norm_equals_rotate_then_append(yahkv, torch_g
         assert torch.equal(getattr(a, name), getattr(b, name)), name
 
 
+def test_many_short_sequences_equal_few(yahkv, torch_gpu):
+    """1200 tokens in one call and in two: the same bytes, query rows and rotated K rows."""
+    torch = torch_gpu
+    n, new, pt = 300, 4, 16
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    g = yahkv.geometry(8, 24, 4, 256, pt, n)
+    whole, parts = yahkv.DevicePools(g, fill=1), yahkv.DevicePools(g, fill=1)
+    qkv = torch.randn(n, new, 32, 256, generator=gen, device="cuda").half()
+    q, k, v = qkv[:, :, :24], qkv[:, :, 24:28], qkv[:, :, 28:]
+    table = torch.randperm(n, generator=gen, device="cuda").to(torch.int32).view(n, 1)
+    start = torch.randint(0, 13, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    pos = torch.randint(0, 100000, (n, new), generator=gen, device="cuda", dtype=torch.int32)
+    r = make(yahkv, 64, "half", "linear", normalise=True)
+    k_out = [torch.zeros(n, new, 4, 256, device="cuda") for _ in range(2)]
+    want = yahkv.rotary_append(whole, table, start, r, k, v, q, positions=pos, k_out=k_out[0])
+    half = [yahkv.rotary_append(parts, table[s], start[s], r, k[s], v[s], q[s], positions=pos[s], k_out=k_out[1][s])
+            for s in (slice(0, 150), slice(150, 300))]
+    assert torch.equal(want, torch.cat(half)) and torch.equal(k_out[0], k_out[1])
+    for name in ("kq", "ks", "vq", "vs"):
+        assert torch.equal(getattr(whole, name), getattr(parts, name)), name
+
+
 def test_replays_from_a_graph_on_another_stream(yahkv, torch_gpu):
     torch = torch_gpu
     g = yahkv.geometry(8, 24, 4, 256, 64, 4)

@@ -53,7 +53,7 @@ struct RopeArgs {
 // What AppendRows does to K and query rows before it stores them.
 enum RowsMode { kAsTheyAre = 0, kNeox = 1, kGeneral = 2 };
 
-// One workgroup of four wavefronts per token. With ROPE, the token's angles (they depend on the position and the
+// One workgroup of four wavefronts per token (or several: FLIGHT below). With ROPE, the token's angles (they depend on the position and the
 // pair, not on the head) are computed once into LDS; without, K rows are quantized as they are (plain append) and
 // there are no query rows. The token's rows of head_dim values (its H K heads, its H V heads, then its
 // query heads) are dealt to the wavefronts in turn; a row lies across a wavefront, four consecutive dims per lane, so
@@ -62,8 +62,11 @@ enum RowsMode { kAsTheyAre = 0, kNeox = 1, kGeneral = 2 };
 // loads of all its rows (up to eight at a time) before it works on the first; for that the loads must not sit behind
 // branches, so the source rows' type SRC is known when compiling (as in AppendPages: with the type a run-time value
 // each load waited for the one before) and a row or lane that has nothing to load asks for an address that exists.
+// FLIGHT: rows whose loads a wavefront issues at a time. Eight fill the memory system in a long call; a short one waits for its
+// code, and its rows go to several workgroups a token (grid y) with one at a time instead (yahkv_rotary_append, 64 tokens of 4
+// + 4 + 24 rows of 256 dims: 5.8 us, with two 6.5, with four 7.4, with eight and one workgroup a token 10).
 constexpr int kRopeWaves = 4, kRowsInFlight = 8;
-template <int FMT, int MODE, int SRC>
+template <int FMT, int MODE, int SRC, int FLIGHT>
 __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) {
 #pragma clang fp contract(off)
   constexpr bool ROPE = MODE != kAsTheyAre;
@@ -152,17 +155,17 @@ __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) 
     else if (row < 2 * H) *src = a.v_src, *off = (tok * H + (row - H)) * D;
     else *src = a.q_src, *off = (tok * g.n_q + (row - 2 * H)) * D;
   };
-  for (int first_row = wave; first_row < rows_per_token; first_row += kRopeWaves * kRowsInFlight) {
-    uint4 raw[kRowsInFlight];
+  for (int first_row = wave + kRopeWaves * FLIGHT * blockIdx.y; first_row < rows_per_token; first_row += kRopeWaves * FLIGHT * gridDim.y) {
+    uint4 raw[FLIGHT];
 #pragma unroll
-    for (int j = 0; j < kRowsInFlight; ++j) {
+    for (int j = 0; j < FLIGHT; ++j) {
       const void* src;
       size_t off;
       source(row_of(min(first_row + kRopeWaves * j, rows_per_token - 1)), &src, &off);
       raw[j] = LoadRaw4(src, off + (has ? d0 : 0), SRC);
     }
 #pragma unroll
-    for (int j = 0; j < kRowsInFlight; ++j) {
+    for (int j = 0; j < FLIGHT; ++j) {
       if (first_row + kRopeWaves * j >= rows_per_token) break;
       const int row = row_of(first_row + kRopeWaves * j);
       const bool is_v = row >= H && row < 2 * H, is_q = row >= 2 * H;
@@ -499,17 +502,17 @@ void LaunchPages(int32_t format, int32_t src_dtype, int32_t n_seqs, int32_t n_ne
     else hipLaunchKernelGGL((AppendPages<4, YAHKV_BF16, TURN>), grid, block, 0, st, a);
   }
 }
-template <int ROPE>
+template <int ROPE, int FLIGHT = kRowsInFlight>
 void LaunchRows(int32_t format, int32_t src_dtype, dim3 grid, hipStream_t st, const RopeArgs& a) {
   const dim3 block(64 * kRopeWaves);
   if (format == YAHKV_Q8_0) {
-    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendRows<8, ROPE, YAHKV_F32>), grid, block, 0, st, a);
-    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendRows<8, ROPE, YAHKV_F16>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((AppendRows<8, ROPE, YAHKV_BF16>), grid, block, 0, st, a);
+    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendRows<8, ROPE, YAHKV_F32, FLIGHT>), grid, block, 0, st, a);
+    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendRows<8, ROPE, YAHKV_F16, FLIGHT>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((AppendRows<8, ROPE, YAHKV_BF16, FLIGHT>), grid, block, 0, st, a);
   } else {
-    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_F32>), grid, block, 0, st, a);
-    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_F16>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_BF16>), grid, block, 0, st, a);
+    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_F32, FLIGHT>), grid, block, 0, st, a);
+    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_F16, FLIGHT>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((AppendRows<4, ROPE, YAHKV_BF16, FLIGHT>), grid, block, 0, st, a);
   }
 }
 // Rows [n_seqs][n_new][n_kv][D] without gaps.
@@ -553,6 +556,13 @@ int LaunchTurned(RopeArgs a, hipStream_t st) {
     a.per_xcd = ((n_new + 7) / 8 + m.pt - 1) / m.pt * m.pt;
     blocks = int64_t(n_seqs) * 8 * a.per_xcd;
     if (blocks > 0x7FFFFFFF) return YAHKV_ERR_SHAPE;
+  }
+  if constexpr (MODE == kGeneral) {
+    if (blocks < 1024) {
+      const int rows = (a.skip_v ? 1 : 2) * m.n_kv + (a.q_src != nullptr ? m.n_q : 0), parts = (rows + kRopeWaves - 1) / kRopeWaves;
+      LaunchRows<MODE, 1>(format, src_dtype, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), st, a);
+      return LaunchStatus();
+    }
   }
   LaunchRows<MODE>(format, src_dtype, dim3(static_cast<unsigned>(blocks)), st, a);
   return LaunchStatus();
