@@ -244,3 +244,10 @@ def test_binding_refuses_tensors_of_another_shape(yahkv):
         yahkv.rotary_rows(yahkv.Rotary(64, 1e4, q_weight=torch.ones(64), device="cpu"), i(3, 1), x)
     with pytest.raises(yahkv.YahkvError):
         yahkv.DevicePools.of(g, dev.kq, dev.ks, dev.vq.view(2, -1).t(), dev.vs)
+
+
+def test_shared_workspace_does_not_grow_with_the_bounds(yahkv):
+    """Bounds far above the lengths cost a bounded number of partials: 64 rows of 16 workgroups for each of 256 compute units."""
+    g = yahkv.geometry(8, 24, 4, 256, 64, 1000)
+    for n, groups, shared, tail in ((1, 1, 0, 2 ** 30), (64, 1, 32768, 2 ** 30), (64, 64, 2 ** 30, 2 ** 30)):
+        assert 0 < yahkv.decode_shared_workspace_bytes(g, n, groups, shared, tail) <= 64 * 16 * 256 * 258 * 4

@@ -626,12 +626,14 @@ SharedPlan MakeSharedPlan(const Geom& m, int32_t n_seqs, int32_t n_groups, int32
   // A prefix is cut so that the row blocks of an average group give every CU a workgroup, or two if its registers hold them
   // and each still has four tiles a wave (256 rows x 32K keys of 128 dims: 95 us, with one 117; 64 rows x 8K: 24 and 20). A
   // tail is cut into pieces of at most sixteen tiles, and finer while that leaves CUs idle; a piece has a tile for every wave.
+  // Sixteen workgroups a CU are enough of them: what a bound far above the lengths costs is their places in the workspace.
   const int64_t per_piece = std::max<int64_t>(1, std::min<int64_t>(int64_t(n_groups) * blocks(p.row_blocks), p.max_blocks)) * m.n_kv;
   const bool two = p.row_blocks * m.hd <= 256 && 2 * cus / per_piece * 4 * 4 <= pre_tiles;
   p.n_split = static_cast<int32_t>(std::max<int64_t>(1, std::min((two ? 2 * cus : cus) / per_piece, (pre_tiles + 3) / 4)));
   if (pre_tiles == 0) p.n_split = 0;
   const int64_t tails = int64_t(n_seqs) * m.n_kv;
-  p.tail_split = static_cast<int32_t>(std::max<int64_t>(1, std::min(std::max((cus + tails - 1) / tails, (tail_tiles + 15) / 16), (tail_tiles + 3) / 4)));
+  const int64_t pieces = std::min(std::max((cus + tails - 1) / tails, (tail_tiles + 15) / 16), std::max<int64_t>(16 * cus / tails, 1));
+  p.tail_split = static_cast<int32_t>(std::max<int64_t>(1, std::min(pieces, (tail_tiles + 3) / 4)));
   p.prefix_groups = static_cast<int32_t>((int64_t(m.n_kv) * p.n_split + 7) / 8 * 8 * p.max_blocks);
   p.groups = p.prefix_groups + tails * p.tail_split;
   const size_t parts = size_t(n_seqs) * m.n_q * (p.n_split + p.tail_split);
