@@ -251,9 +251,11 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
 
   __shared__ __align__(16) uint8_t lk[8 * 64 * 32], lv[256 * (64 + 4)];  // images of the K and V code regions
   __shared__ __align__(16) uint16_t lks[64 * 8], lvs[8 * 64];      // and of the scale regions
-  const int d0 = 4 * lane, b = lane / 8, lb = lane % 8;
-  const bool has = d0 < D;
-  // A wavefront takes four consecutive tokens at a time (their rows in flight together): a lane then holds, for each
+  // A row lies across D / 4 lanes, so that at 128 dims a wavefront has two sets of four tokens side by side (5 x 1037 tokens of 8
+  // heads, pages of 32: 14.4 us, turned 24.4; with half the lanes idle 18.9 and 31.6).
+  const int row_lanes = D / 4, sets = 64 / row_lanes, set = lane / row_lanes, rl = lane % row_lanes;
+  const int d0 = 4 * rl, b = rl / 8, lb = rl % 8;
+  // A set of lanes takes four consecutive tokens at a time (their rows in flight together): a lane then holds, for each
   // of its four dims, the codes of four neighbouring tokens, which is one dword of the V image instead of four bytes.
   // (The image's rows are padded by a dword: with rows of exactly PT bytes the 64 lanes of such a store would all
   // hit one LDS bank.)
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
     for (int j = 0; j < 4; ++j) {
       const int t = 4 * q + j;
       rk[j] = rv[j] = uint4{0u, 0u, 0u, 0u};  // reads as 0.0 in every source type
-      if (t >= t_lo && t < t_hi && has) {
+      if (t >= t_lo && t < t_hi) {
         const int tok = token_at(pi * PT + t);
         rv[j] = LoadRaw4(a.v_src, static_cast<size_t>(s * a.v_rows.seq + tok * a.v_rows.token + h * a.v_rows.head) + d0, SRC);
         if (!a.skip_k) {
@@ -274,29 +276,30 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
       }
     }
   };
-  __shared__ __align__(16) float lcs[TURN ? kPageWaves : 1][4][TURN ? 128 : 4], lsn[TURN ? kPageWaves : 1][4][TURN ? 128 : 4];
+  __shared__ __align__(16) float lcs[TURN ? kPageWaves : 1][TURN ? 512 : 4], lsn[TURN ? kPageWaves : 1][TURN ? 512 : 4];
+  auto angle = [&](int j, int p) -> int { return (4 * set + j) * (D / 2) + p; };  // place of pair p of the set's token j
   float4 wk = {1.0f, 1.0f, 1.0f, 1.0f};
   if constexpr (TURN)
-    if (a.k_weight != nullptr && has) wk = *reinterpret_cast<const float4*>(a.k_weight + d0);
-  // the K rows of tokens 4 q .. 4 q + 3, normalised and turned (see AppendRows for a lane's part of the rotation)
+    if (a.k_weight != nullptr) wk = *reinterpret_cast<const float4*>(a.k_weight + d0);
+  // the K rows of the set's tokens 4 q .. 4 q + 3, normalised and turned (see AppendRows for a lane's part of the rotation)
   auto turn = [&](int q, float4 (&kx)[4]) {
     const int rot = a.rotary.rot, half = rot / 2, r0 = d0 - a.rotary.first;
-    const bool turned = has && r0 >= 0 && r0 < rot, inside = a.rotary.layout == YAHKV_ROTARY_INTERLEAVED, first = r0 < half;
+    const bool turned = r0 >= 0 && r0 < rot, inside = a.rotary.layout == YAHKV_ROTARY_INTERLEAVED, first = r0 < half;
     const int partner = turned && !inside ? (first ? lane + half / 4 : lane - half / 4) : lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int t = min(max(4 * q + j, t_lo), t_hi - 1), tok = token_at(pi * PT + t);
       const int pos = a.positions != nullptr ? a.positions[static_cast<int64_t>(s) * a.n_new + tok] : start + tok;
-      for (int p = lane; p < half; p += 64) {
+      for (int p = rl; p < half; p += row_lanes) {
         float c, v;
         TurnCosSin(pos, a.rotary.turns[p], &c, &v);
-        lcs[wave][j][p] = c * a.rotary.magnitude, lsn[wave][j][p] = v * a.rotary.magnitude;
+        lcs[wave][angle(j, p)] = c * a.rotary.magnitude, lsn[wave][angle(j, p)] = v * a.rotary.magnitude;
       }
     }
     if (a.rotary.normalise) {
       float ss[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ss[j] = WaveSum(kx[j].x * kx[j].x + kx[j].y * kx[j].y + kx[j].z * kx[j].z + kx[j].w * kx[j].w);
+      for (int j = 0; j < 4; ++j) ss[j] = RowSum(kx[j].x * kx[j].x + kx[j].y * kx[j].y + kx[j].z * kx[j].z + kx[j].w * kx[j].w, sets == 1);
       // (lane l works out the reciprocal of row l % 4 for everybody)
       const float mine = lane & 2 ? (lane & 1 ? ss[3] : ss[2]) : (lane & 1 ? ss[1] : ss[0]);
       const float inv = 1.0f / sqrtf(mine / static_cast<float>(D) + a.eps);
@@ -314,12 +317,12 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
       float4 x;
       if (inside) {
         const int p = turned ? r0 / 2 : 0;
-        const float2 c = *reinterpret_cast<const float2*>(&lcs[wave][j][p]), sv = *reinterpret_cast<const float2*>(&lsn[wave][j][p]);
+        const float2 c = *reinterpret_cast<const float2*>(&lcs[wave][angle(j, p)]), sv = *reinterpret_cast<const float2*>(&lsn[wave][angle(j, p)]);
         x = float4{v.x * c.x - v.y * sv.x, v.y * c.x + v.x * sv.x, v.z * c.y - v.w * sv.y, v.w * c.y + v.z * sv.y};
       } else {
         const int p = turned ? (first ? r0 : r0 - half) : 0;
-        const float4 c = *reinterpret_cast<const float4*>(&lcs[wave][j][p]);
-        float4 sv = *reinterpret_cast<const float4*>(&lsn[wave][j][p]);
+        const float4 c = *reinterpret_cast<const float4*>(&lcs[wave][angle(j, p)]);
+        float4 sv = *reinterpret_cast<const float4*>(&lsn[wave][angle(j, p)]);
         if (first) sv = float4{-sv.x, -sv.y, -sv.z, -sv.w};
         const float px = __shfl(v.x, partner, 64), py = __shfl(v.y, partner, 64);
         const float pz = __shfl(v.z, partner, 64), pw = __shfl(v.w, partner, 64);
@@ -329,12 +332,15 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
     }
     __builtin_amdgcn_wave_barrier();  // (the table is rewritten for the next four tokens)
   };
-  if (4 * (t_lo / 4 + wave) < t_hi) request(t_lo / 4 + wave);
-  for (int q = t_lo / 4 + wave; 4 * q < t_hi; q += kPageWaves) {
+  const int span = 4 * sets;  // tokens of a wavefront at a time (pages are multiples of 16)
+  int w0 = t_lo / span + wave;
+  if (span * w0 < t_hi) request(sets * w0 + set);
+  for (; span * w0 < t_hi; w0 += kPageWaves) {
+    const int q = sets * w0 + set;
     float4 kx[4], vx[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) kx[j] = Widen4(rk[j], SRC), vx[j] = Widen4(rv[j], SRC);
-    if (4 * (q + kPageWaves) < t_hi) request(q + kPageWaves);
+    if (span * (w0 + kPageWaves) < t_hi) request(q + sets * kPageWaves);
     if constexpr (TURN) turn(q, kx);
     uint32_t vc[4];
     if constexpr (FMT == 8) {
@@ -352,7 +358,7 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
       ScaleQ8(mine, &inv, &sc);
       {
         const int t = 4 * q + lb % 4;  // row lb is K (lb < 4) or V of this token
-        if (has && t >= t_lo && t < t_hi) {
+        if (t >= t_lo && t < t_hi) {
           if (lb < 4) lks[t * NB + b] = sc;
           else lvs[b * PT + t] = sc;
         }
@@ -362,7 +368,7 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
         const int t = 4 * q + j;
         const uint32_t kc = CodesLanesQ8(kx[j], __shfl(inv, (lane & ~7) | j, 64));
         vc[j] = CodesLanesQ8(vx[j], __shfl(inv, (lane & ~7) | (4 + j), 64));
-        if (!has || t < t_lo || t >= t_hi) continue;
+        if (t < t_lo || t >= t_hi) continue;
         *reinterpret_cast<uint32_t*>(&lk[(b * PT + t) * KB + 4 * lb]) = kc;
       }
     } else {
@@ -372,12 +378,12 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
         uint16_t ksc, vsc;
         const uint32_t kc = QuantizeLanesQ4(kx[j], lb, &ksc);
         vc[j] = QuantizeLanesQ4(vx[j], lb, &vsc);
-        if (!has || t < t_lo || t >= t_hi) continue;
+        if (t < t_lo || t >= t_hi) continue;
         if (lb == 0) lks[t * NB + b] = ksc, lvs[b * PT + t] = vsc;
         if (lb < 4) *reinterpret_cast<uint32_t*>(&lk[(b * PT + t) * KB + 4 * lb]) = kc;
       }
     }
-    if (has && (FMT == 8 || lb < 4)) {
+    if (FMT == 8 || lb < 4) {
       const int r0 = FMT == 8 ? d0 : b * 16 + 4 * lb;  // this lane's four byte rows of the V image
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -533,7 +539,7 @@ int LaunchTurned(RopeArgs a, hipStream_t st) {
     // The general rotation has K page by page as well, unless the caller wants the rotated rows of every token (those that
     // clamp to a slot another token takes are not visited there), and the query rows by the rows kernel, which has eight
     // dims a lane and several rows a wave where AppendRows has four and one (5 x 1037 tokens of 32 + 8 heads of 128 dims:
-    // 101 -> 57 us).
+    // 101 -> 47 us).
     const bool k_pages = MODE == kGeneral && a.k_out == nullptr;
     RopeArgs v = a;
     v.skip_k = !k_pages;

@@ -59,9 +59,9 @@ __device__ __forceinline__ float LaneXor(float x) {
   return __builtin_bit_cast(float, LaneXorBits<K>(__builtin_bit_cast(uint32_t, x)));
 }
 
-// Sum over the 64 lanes, in every lane: four DPP steps inside each row of 16 lanes, then the two row-swapping
-// instructions of gfx950 across the rows (no LDS round trips).
-__device__ __forceinline__ float WaveSum(float v) {
+// Sum over all 64 lanes of a wave (`whole`), or over each half of it, in every lane: four DPP steps inside each row of 16 lanes,
+// then the two row-swapping instructions of gfx950 across the rows (no LDS round trips).
+__device__ __forceinline__ float RowSum(float v, bool whole) {
   v += Dpp<kQuadSwap1>(v);
   v += Dpp<kQuadSwap2>(v);
   v += Dpp<kHalfMirror>(v);
@@ -70,11 +70,13 @@ __device__ __forceinline__ float WaveSum(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   const uint32_t r0 = r[0], r1 = r[1];
   const float w = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+  if (!whole) return w;
   const uint32_t x = __builtin_bit_cast(uint32_t, w);
   const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   const uint32_t q0 = q[0], q1 = q[1];
   return __builtin_bit_cast(float, q0) + __builtin_bit_cast(float, q1);
 }
+__device__ __forceinline__ float WaveSum(float v) { return RowSum(v, true); }
 
 // A block of 32 values lies in 8 consecutive lanes, 4 values each (lane l of the 8: elements 4 l .. 4 l + 3).
 // q8_0: the block's amax in all 8 lanes (a maximum does not depend on the order), then the scalar formulas of
