@@ -454,7 +454,8 @@ int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* pools, const
  *              tail) and of the tokens any sequence reads through its own row (more are cut off, as lengths above
  *              max_seq_len are elsewhere)
  * softmax_scale > 0. Two dispatches, the partials of prefixes and tails and their merge, or three: tails that fill the GPU
- * have one of their own. */
+ * have one of their own. The workspace needs no preparation and holds nothing between calls; calls that may run at the same
+ * time, replays of captured graphs among them, need one each. */
 size_t yahkv_decode_shared_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t n_groups, int32_t max_shared_len,
                                            int32_t max_tail_len);
 int yahkv_decode_attend_shared(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
@@ -470,7 +471,7 @@ int yahkv_decode_attend_shared(const yahkv_geometry* g, const yahkv_pools* pools
  * with f32 rows [n_seqs][n_kv_heads][weights_stride]; weights_in may be NULL (zeros) or weights_out itself; entries at or
  * past the length are not touched (a new token's entry is read in its first step: clear the rows before a sequence begins). out is of out_dtype (F32, F16 or BF16); other arguments as yahkv_decode_attend. The weights
  * are f32 throughout (scores from the exact codes), whatever out_dtype; lengths above max_seq_len or above weights_stride
- * are clamped, and max_seq_len may not exceed weights_stride. Three dispatches. */
+ * are clamped, and max_seq_len may not exceed weights_stride. Three dispatches; the workspace as for the shared prefixes. */
 size_t yahkv_decode_weights_workspace_bytes(const yahkv_geometry* g, int32_t n_seqs, int32_t max_seq_len);
 int yahkv_decode_attend_weights(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t* page_table,
                                 int32_t page_table_stride, const int32_t* seq_len, int32_t n_seqs, int32_t max_seq_len,

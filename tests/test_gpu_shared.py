@@ -200,6 +200,39 @@ def test_same_bits_twice_and_from_a_graph(yahkv, torch_gpu):
         a["seq_len"].sub_(i)
 
 
+def test_two_graphs_on_one_workspace(yahkv, torch_gpu):
+    """A shared step and a weighing step, captured apart on the same workspace and replayed in turn: what each gives alone."""
+    torch = torch_gpu
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 24, 4, 256, 64, [(640, [650, 700, 900]), (0, [70])], 12)
+    q = q.half()
+    need = max(yahkv.decode_shared_workspace_bytes(dev.geom, 4, 2, a["max_shared_len"], a["max_tail_len"]),
+               yahkv.decode_weights_workspace_bytes(dev.geom, 4, 900))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    out, w = torch.empty(4, 24, 256, device="cuda"), torch.zeros(4, 4, 900, device="cuda")
+    out2 = torch.empty_like(out)
+    steps = [lambda: yahkv.decode_attend_shared(dev, q=q, scale=0.0625, out=out, workspace=ws, **a),
+             lambda: yahkv.decode_attend_weights(dev, a["table"], a["seq_len"], 900, q, 0.0625, w, out=out2, workspace=ws)]
+    for s in steps:
+        s()
+    want = out.clone(), w.clone(), out2.clone()
+    graphs, stream = [torch.cuda.CUDAGraph() for _ in steps], torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for graph, s in zip(graphs, steps):
+            with torch.cuda.graph(graph, stream=stream):
+                s()
+    for i in range(3):
+        for x in (out, w, out2):
+            x.fill_(-1.0)
+        torch.cuda.synchronize()
+        for graph in (graphs if i % 2 else graphs[::-1]):
+            graph.replay()
+        torch.cuda.synchronize()
+        for s, n in enumerate(lens):
+            assert torch.equal(w[s, :, :n], want[1][s, :, :n])
+        assert torch.equal(out, want[0]) and torch.equal(out2, want[2]), i
+
+
 def test_workspace_too_small_is_refused(yahkv, torch_gpu):
     torch = torch_gpu
     g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, 8, 2, 128, 16, [(64, [70])], 9)
