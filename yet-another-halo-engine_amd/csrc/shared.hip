@@ -551,7 +551,7 @@ __global__ __launch_bounds__(64 * kSharedWaves, RB * D <= 256 ? 2 : 1) void Shar
 
 // One workgroup per (query head, sequence): the prefix's partials and the tail's, weighed by 2^(m - M) and 1 / l. A group of
 // D / 4 lanes takes every n-th partial, four dims a lane; the groups' sums meet in LDS. (64 x 24 rows of up to ten partials of 256
-// dims: 6.9 us, a round trip behind a round trip; the partials are in the caches.)
+// dims: 6.0 us, a round trip behind a round trip; the partials are in the caches.)
 struct MergeArgs {
   SharedArgs s;
   const float* gate;
@@ -572,6 +572,16 @@ __global__ __launch_bounds__(kMergeThreads) void SharedMerge(const MergeArgs a) 
   __shared__ float red[kMergeThreads / 64];
   __shared__ __align__(16) float sums[kMergeThreads * 4];
   __shared__ float lsum[kMergeThreads / 32];
+  const int lanes = D / 4, grp = t / lanes, dl = t % lanes, groups = kMergeThreads / lanes;
+  auto sum_of = [&](int i) { return *reinterpret_cast<const float2*>(&a.s.ml[slot_of(i) * 2]); };
+  auto acc_of = [&](int i) { return *reinterpret_cast<const float4*>(&a.s.acc[slot_of(i) * D + 4 * dl]); };
+  // (a lane's first partials are asked for before the maximum is known: one round trip less)
+  constexpr int kEarly = 4;
+  float2 v0[kEarly];
+  float4 x0[kEarly];
+#pragma unroll
+  for (int e = 0; e < kEarly; ++e)
+    if (grp + e * groups < n) v0[e] = sum_of(grp + e * groups), x0[e] = acc_of(grp + e * groups);
   float M = kNegMax;
   for (int i = t; i < n; i += kMergeThreads) M = fmaxf(M, a.s.ml[slot_of(i) * 2]);
   M = WaveMax(M);
@@ -579,19 +589,19 @@ __global__ __launch_bounds__(kMergeThreads) void SharedMerge(const MergeArgs a) 
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kMergeThreads / 64; ++w) M = fmaxf(M, red[w]);
-  const int lanes = D / 4, grp = t / lanes, dl = t % lanes, groups = kMergeThreads / lanes;
   float4 A = {0.0f, 0.0f, 0.0f, 0.0f};
   float L = 0.0f;
-#pragma unroll 4
-  for (int i = grp; i < n; i += groups) {
-    const size_t at = slot_of(i);
-    const float2 v = *reinterpret_cast<const float2*>(&a.s.ml[at * 2]);
-    const float4 x = *reinterpret_cast<const float4*>(&a.s.acc[at * D + 4 * dl]);
+  auto add = [&](const float2 v, const float4 x) {
     const float w = __builtin_amdgcn_exp2f(v.x - M);
     A.x = __builtin_fmaf(w, x.x, A.x), A.y = __builtin_fmaf(w, x.y, A.y);
     A.z = __builtin_fmaf(w, x.z, A.z), A.w = __builtin_fmaf(w, x.w, A.w);
     L = __builtin_fmaf(w, v.y, L);
-  }
+  };
+#pragma unroll
+  for (int e = 0; e < kEarly; ++e)
+    if (grp + e * groups < n) add(v0[e], x0[e]);
+#pragma unroll 4
+  for (int i = grp + kEarly * groups; i < n; i += groups) add(sum_of(i), acc_of(i));
   *reinterpret_cast<float4*>(&sums[grp * D + 4 * dl]) = A;
   if (dl == 0) lsum[grp] = L;
   __syncthreads();
