@@ -105,7 +105,7 @@ def test_lengths_and_groups(yahkv, torch_gpu, groups):
 
 
 @pytest.mark.parametrize("fmt,pt", [(8, 64), (8, 32), (8, 16), (4, 64), (4, 32), (4, 16)])
-@pytest.mark.parametrize("n_q,n_kv,hd", [(24, 4, 256), (32, 8, 128)])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(24, 4, 256), (32, 8, 128), (8, 1, 256), (5, 1, 128)])
 def test_bounds_of_a_large_call(yahkv, torch_gpu, n_q, n_kv, hd, fmt, pt):
     """The host bounds of a long context choose as many row blocks a wave as registers hold, and tails in a launch of their
     own, whatever the lengths on the device are."""
