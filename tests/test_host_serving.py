@@ -251,3 +251,13 @@ def test_shared_workspace_does_not_grow_with_the_bounds(yahkv):
     g = yahkv.geometry(8, 24, 4, 256, 64, 1000)
     for n, groups, shared, tail in ((1, 1, 0, 2 ** 30), (64, 1, 32768, 2 ** 30), (64, 64, 2 ** 30, 2 ** 30)):
         assert 0 < yahkv.decode_shared_workspace_bytes(g, n, groups, shared, tail) <= 64 * 16 * 256 * 258 * 4
+
+
+def test_output_types_are_refused(yahkv):
+    import torch
+    q = torch.zeros(1, 8, 128, dtype=torch.float16)
+    with pytest.raises(yahkv.YahkvError):
+        yahkv._out(None, q, torch.int32, torch.float32)
+    with pytest.raises(yahkv.YahkvError):
+        yahkv._out(torch.zeros(1, 8, 128, dtype=torch.int32), q, None, torch.float32)
+    assert yahkv._out(None, q.transpose(1, 2), torch.bfloat16, torch.float32).is_contiguous()

@@ -690,7 +690,7 @@ def _run_on(device, call, what):
     if device.type != "cuda":
         _refuse(f"{what}: tensors on a GPU are expected")
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():  # (tensors are there, so the runtime is up)
         status = call(torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
@@ -699,12 +699,19 @@ def _run_on(device, call, what):
         raise YahkvError(status, what)
 
 
-def _out(out, shape, dtype, device, default):
-    """The caller's output tensor after a look at it, or a new one."""
+def _new(like, dtype):  # (half the host time of torch.empty with a shape and a device)
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _out(out, like, dtype, default):
+    """The caller's output tensor, of the shape and device of `like`, after a look at it, or a new one."""
     if out is None:
-        return torch.empty(shape, dtype=dtype or default, device=device)
-    if out.shape != shape or not out.is_contiguous() or out.device != device or dtype not in (None, out.dtype) or out.dtype not in _DTYPES:
-        _refuse(f"out: a contiguous tensor of shape {tuple(shape)} on {device} is expected")
+        if dtype is not None and dtype not in _DTYPES:
+            _refuse(f"out_dtype: {dtype}")
+        return _new(like, dtype or default)
+    if (out.shape != like.shape or not out.is_contiguous() or out.device != like.device or dtype not in (None, out.dtype) or
+            out.dtype not in _DTYPES):
+        _refuse(f"out: a contiguous tensor of shape {tuple(like.shape)} on {like.device} is expected")
     return out
 
 
@@ -764,10 +771,10 @@ def _rows(t, what):
     return Rows(t.data_ptr(), code, heads, a if n > 1 else 0, b if new > 1 else 0, c if heads > 1 else 0)
 
 
-def _new_rows(shape, dtype, device):
+def _new_rows(like, dtype):
     """A new contiguous tensor of the (checked) rows' shape, and it as yahkv_rows."""
-    t = torch.empty(shape, dtype=dtype, device=device)
-    _, new, heads, d = shape
+    t = _new(like, dtype)
+    _, new, heads, d = like.shape
     return t, Rows(t.data_ptr(), _DTYPES[dtype], heads, new * heads * d, heads * d, d)
 
 
@@ -802,7 +809,7 @@ def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_d
         if out is None:
             if dtype not in _DTYPES:
                 _refuse(f"rotary_rows: out_dtype {dtype}")
-            out, dst = _new_rows(shape, dtype, dev)
+            out, dst = _new_rows(x, dtype)
         else:
             if out.shape != shape or out.device != dev:
                 _refuse("rotary_rows: out has the rows' shape")
@@ -839,7 +846,7 @@ def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None,
         qs = _rows(q, "q")
         if q_out is None:
             _need(q_out_dtype is None or q_out_dtype in _DTYPES, "rotary_append: q_out_dtype")
-            q_out, qd = _new_rows(q.shape, q_out_dtype or torch.float32, dev)
+            q_out, qd = _new_rows(q, q_out_dtype or torch.float32)
         else:
             _need(q_out.shape == q.shape and q_out.device == dev, "rotary_append: q_out has q's shape")
             qd = _rows(q_out, "q_out")
@@ -873,7 +880,7 @@ def decode_attend_shared(pools, table, seq_len, group_first, shared_len, max_sha
     n_groups = shared_len.shape[0]
     _ints(shared_len, (n_groups,), dev, "shared_len")
     _ints(group_first, (n_groups + 1,), dev, "group_first")
-    out = _out(out, q.shape, out_dtype, dev, torch.float32)
+    out = _out(out, q, out_dtype, torch.float32)
     workspace = _scratch(workspace, lambda: decode_shared_workspace_bytes(g, n_seqs, n_groups, max_shared_len, max_tail_len), dev)
     st = pools.struct()
     _run_on(dev, lambda stream: lib.yahkv_decode_attend_shared(
@@ -906,7 +913,7 @@ def decode_attend_weights(pools, table, seq_len, max_seq_len, q, scale, weights_
     _weight_rows(weights_out, g, n_seqs, max_seq_len, dev, "weights_out")
     _need(weights_in is None or (weights_in.shape == weights_out.shape and weights_in.dtype == torch.float32 and
                                  weights_in.is_contiguous() and weights_in.device == dev), "weights_in: as weights_out")
-    out = _out(out, q.shape, out_dtype, dev, torch.float32)
+    out = _out(out, q, out_dtype, torch.float32)
     workspace = _scratch(workspace, lambda: decode_weights_workspace_bytes(g, n_seqs, max_seq_len), dev)
     st = pools.struct()
     _run_on(dev, lambda stream: lib.yahkv_decode_attend_weights(
