@@ -239,3 +239,30 @@ def test_workspace_too_small_is_refused(yahkv, torch_gpu):
     with pytest.raises(yahkv.YahkvError) as e:
         yahkv.decode_attend_shared(dev, q=q, scale=0.1, workspace=torch.empty(64, dtype=torch.uint8, device="cuda"), **a)
     assert e.value.status == -4
+
+
+@pytest.mark.parametrize("fmt,n_q,n_kv,hd,pt,big", [(8, 24, 4, 256, 64, 60000.0), (8, 8, 2, 128, 16, 600.0), (8, 32, 8, 128, 32, 65504.0),
+                                                    (4, 24, 4, 256, 32, 60000.0), (4, 8, 2, 128, 64, 9000.0)])
+@pytest.mark.parametrize("bound", [0, 65536])
+def test_keys_beyond_the_f16_range(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, big, bound):
+    """Keys whose values d * code are far beyond 65504, in prefixes and tails, next to ordinary ones: their scores are the plain
+    decode attention's. The softmax scale brings the large ones' scores to a standard deviation of about four."""
+    torch = torch_gpu
+    groups = [(192, [192, 250, 300, 0]), (0, [70]), (640, [700] * 30)]
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, fmt, n_q, n_kv, hd, pt, groups, int(big) + hd)
+    ks = dev.ks.view(torch.float16).view(-1, n_kv, pt, hd // 32)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    some = torch.rand(ks.shape[:3], generator=gen, device="cuda") < 0.3
+    blocks = torch.rand(ks.shape, generator=gen, device="cuda")
+    large = ((0.5 + 0.5 * blocks) * big).half()
+    ks.copy_(torch.where(some[..., None] & (blocks > 0.25) & torch.isfinite(ks), large, ks))
+    for name, arr in host.arrays().items():
+        arr.reshape(-1)[:] = dev.numpy()[name].reshape(-1)
+    rms = {8: 45.0, 4: 3.0}[fmt] * 0.75 * big                          # of a large key's values
+    scale = 4.0 / (rms * hd ** 0.5)
+    if bound:
+        a.update(max_shared_len=bound, max_tail_len=40000)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), scale)
+    plain = yahkv.decode_attend(dev, a["table"], a["seq_len"], max(lens), q.half(), scale)
+    check(torch, plain, want, torch.float32)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=scale, **a), want, torch.float32)

@@ -17,7 +17,8 @@
 // holds after the four key tiles are those of keys 16 jg .. 16 jg + 15, the ones its V load has. P never leaves its lane.
 // A register is asked for again (for the wave's next tile) as soon as its codes are decoded, so a load has about a tile's
 // time to arrive, without a barrier anywhere in the loop. Decoding is packed f16 arithmetic, perm, add, multiply for two
-// values, the product d * code rounded once and saturated at the largest finite f16 (SetSaturation).
+// values, the product d * code rounded once; beyond the f16 range V's saturates (SetSaturation), K's takes a power of two
+// (ShrinkLargeKeys).
 // Roundings to f16 (11 bits): queries given as f32, K, V and the numerators, each once; products and sums are f32. With scores
 // of a standard deviation of two K's costs 3.5e-4 of the output's norm, the numerators' 2.0e-4, V's 1.6e-4 (an f16 output's own
 // is 2.1e-4). Exact K codes with their scales on the sums instead would take 12 multiplications for every 4 saved here with
@@ -106,20 +107,35 @@ __device__ __forceinline__ float OverLaneGroups(float v, Op op) {
   return op(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
 }
 
-// Products d * code beyond the f16 range saturate (they would be infinite, and an infinite score a NaN). MODE.FP16_OVFL
-// (bit 23) does that in the multiply for nothing, but while it is set the matrix unit drops NaN operands, so it is set for
-// the tiles that need it alone: those with a scale above 511 (128 x 511 is below the largest f16) and none that is not
-// finite. k, v: the tile's scales, eight and eight a lane.
-__device__ __forceinline__ void SetSaturation(const uint4 k, const uint4 v) {
-  typedef uint16_t u2 __attribute__((ext_vector_type(2)));
-  auto mag = [](uint32_t w) { return __builtin_bit_cast(u2, w & 0x7FFF7FFFu); };
-  u2 x = __builtin_elementwise_max(mag(k.x), mag(v.x));
-  x = __builtin_elementwise_max(x, __builtin_elementwise_max(mag(k.y), mag(v.y)));
-  x = __builtin_elementwise_max(x, __builtin_elementwise_max(mag(k.z), mag(v.z)));
-  x = __builtin_elementwise_max(x, __builtin_elementwise_max(mag(k.w), mag(v.w)));
-  const uint32_t most = x[0] > x[1] ? x[0] : x[1];
-  const bool large = __builtin_amdgcn_ballot_w64(most > 0x5FFCu) != 0, finite = __builtin_amdgcn_ballot_w64(most >= 0x7C00u) == 0;
+// Products d * code pass the f16 range where a scale is above 511.75 (128 x 511.75 is the largest f16).
+constexpr uint32_t kLargeScale = 0x5FFF;
+typedef uint16_t us2v __attribute__((ext_vector_type(2)));
+// The larger magnitudes of two pairs of f16 values, as bits.
+__device__ __forceinline__ us2v Magnitudes(uint32_t a, uint32_t b) {
+  return __builtin_elementwise_max(__builtin_bit_cast(us2v, a & 0x7FFF7FFFu), __builtin_bit_cast(us2v, b & 0x7FFF7FFFu));
+}
+__device__ __forceinline__ uint32_t Larger(us2v x) { return x[0] > x[1] ? x[0] : x[1]; }
+
+// V's saturate. MODE.FP16_OVFL (bit 23) does that in the multiply for nothing, but while it is set the matrix unit drops NaN
+// operands, so it is set for the tiles that need it alone: those with a large scale and none that is not finite. v: the
+// tile's scales, eight a lane.
+__device__ __forceinline__ void SetSaturation(const uint4 v) {
+  const uint32_t most = Larger(__builtin_elementwise_max(Magnitudes(v.x, v.y), Magnitudes(v.z, v.w)));
+  const bool large = __builtin_amdgcn_ballot_w64(most > kLargeScale) != 0, finite = __builtin_amdgcn_ballot_w64(most >= 0x7C00u) == 0;
   __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, __builtin_amdgcn_readfirstlane(large && finite ? 1 : 0));
+}
+
+// K's do not: a saturated product would be another score, and an infinite one a NaN. A tile with a large scale enters the
+// product with all its scales times 2^-7, and its scores are multiplied by 2^7 behind it. That is exact but for scales below
+// 2^-7, those of ordinary keys in such a tile, which become whole multiples of 2^-24: 2^-18 off at most, which is to keys of
+// values about one what f16's rounding of them is. k: the tile's scales, eight a lane (those of keys behind the end may be
+// anything: what they hold costs this path and changes nothing). Returns whether it is such a tile.
+__device__ __forceinline__ bool ShrinkLargeKeys(uint4& k) {
+  const uint32_t most = Larger(__builtin_elementwise_max(Magnitudes(k.x, k.y), Magnitudes(k.z, k.w)));
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kLargeScale) == 0, 1)) return false;
+  const _Float16 s = static_cast<_Float16>(0x1p-7f);
+  k = __builtin_bit_cast(uint4, __builtin_bit_cast(h8v, k) * h8v{s, s, s, s, s, s, s, s});
+  return true;
 }
 
 // A barrier behind LDS accesses alone: __syncthreads() would wait for the loads on their way in as well.
@@ -311,6 +327,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
     for (int j = 0; j < PPT; ++j) pgc[j] = pgn[j];
     load_pages(tile + step < tile1 ? tile + step : tile, pgn);
     const bool cut = (tile + 1) * kTile > n_keys;
+    int up = 0;  // this tile's scores come times 2^-up
     {  // scales to LDS; the V scales of masked keys become 0, which makes their V rows 0 whatever they hold
       uint32_t w[4] = {vsr.x, vsr.y, vsr.z, vsr.w};
       if (cut) {
@@ -319,11 +336,12 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
         for (int e = 0; e < 8; ++e)
           if (k0 + e >= n_keys) w[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
       }
+      if (ShrinkLargeKeys(ksr)) up = 7;
       if (lane < NB * 8) {
         *reinterpret_cast<uint4*>(&lds.k[lane * 8]) = ksr;
         *reinterpret_cast<uint4*>(&lds.v[lane * 8]) = uint4{w[0], w[1], w[2], w[3]};
       }
-      SetSaturation(ksr, uint4{w[0], w[1], w[2], w[3]});
+      SetSaturation(uint4{w[0], w[1], w[2], w[3]});
     }
     load_scales(pgn);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -358,6 +376,8 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    asm volatile("" : "+s"(up));  // (a whole number in a scalar register till here: the scale itself would take a vector register)
+    const float tscale = __builtin_ldexpf(sscale, up);
     h8v pv[RB][2];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
@@ -368,7 +388,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
           for (int r = 0; r < 4; ++r)
             if (tile * kTile + 16 * jg + 4 * kt + r >= n_keys) st[i][kt][r] = kNegMax;
       }
-      Numerators<D>(st[i], sscale, m[i], l[i], o[i], pv[i]);
+      Numerators<D>(st[i], tscale, m[i], l[i], o[i], pv[i]);
     }
     // ---- O^T
 #pragma unroll
