@@ -266,3 +266,24 @@ def test_keys_beyond_the_f16_range(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, big
     plain = yahkv.decode_attend(dev, a["table"], a["seq_len"], max(lens), q.half(), scale)
     check(torch, plain, want, torch.float32)
     check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=scale, **a), want, torch.float32)
+
+
+@pytest.mark.parametrize("fmt,hd,pt", [(8, 256, 64), (8, 128, 16), (4, 128, 64), (4, 256, 32)])
+@pytest.mark.parametrize("large", ["ks", "vs", "both"])
+def test_nan_and_infinite_queries_give_nan_beside_large_scales(yahkv, torch_gpu, fmt, hd, pt, large):
+    """What a query's own values make of its row does not depend on the magnitude of the keys and values it meets."""
+    torch = torch_gpu
+    groups = [(192, [192, 250, 300]), (0, [70])]
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, fmt, 8, 2, hd, pt, groups, hd + pt)
+    for name in ("ks", "vs"):
+        if large in (name, "both"):
+            s = getattr(dev, name).view(torch.float16)
+            s.copy_(torch.where(torch.isfinite(s), torch.full_like(s, 60000.0), s))
+    q = q.half()
+    bad = {(0, 3): float("nan"), (2, 5): float("inf"), (3, 0): float("nan")}
+    for (s, h), v in bad.items():
+        q[s, h, 7 * h + 1] = v
+    out = yahkv.decode_attend_shared(dev, q=q, scale=1e-7, **a)
+    for s in range(4):
+        for h in range(8):
+            assert (torch.isnan(out[s, h]) if (s, h) in bad else torch.isfinite(out[s, h])).all(), (s, h)

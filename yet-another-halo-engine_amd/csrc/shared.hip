@@ -17,7 +17,7 @@
 // holds after the four key tiles are those of keys 16 jg .. 16 jg + 15, the ones its V load has. P never leaves its lane.
 // A register is asked for again (for the wave's next tile) as soon as its codes are decoded, so a load has about a tile's
 // time to arrive, without a barrier anywhere in the loop. Decoding is packed f16 arithmetic, perm, add, multiply for two
-// values, the product d * code rounded once; beyond the f16 range V's saturates (SetSaturation), K's takes a power of two
+// values, the product d * code rounded once; beyond the f16 range V's saturates (Saturates), K's takes a power of two
 // (ShrinkLargeKeys).
 // Roundings to f16 (11 bits): queries given as f32, K, V and the numerators, each once; products and sums are f32. With scores
 // of a standard deviation of two K's costs 3.5e-4 of the output's norm, the numerators' 2.0e-4, V's 1.6e-4 (an f16 output's own
@@ -117,12 +117,18 @@ __device__ __forceinline__ us2v Magnitudes(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t Larger(us2v x) { return x[0] > x[1] ? x[0] : x[1]; }
 
 // V's saturate. MODE.FP16_OVFL (bit 23) does that in the multiply for nothing, but while it is set the matrix unit drops NaN
-// operands, so it is set for the tiles that need it alone: those with a large scale and none that is not finite. v: the
-// tile's scales, eight a lane.
-__device__ __forceinline__ void SetSaturation(const uint4 v) {
+// operands: it is set for the second product alone (a NaN among the numerators is in their sum as well, a NaN score
+// would be lost), and only for tiles that need it, those with a large scale and none that is not finite. v: the tile's
+// scales, eight a lane. Returns whether it is such a tile.
+__device__ __forceinline__ bool Saturates(const uint4 v) {
   const uint32_t most = Larger(__builtin_elementwise_max(Magnitudes(v.x, v.y), Magnitudes(v.z, v.w)));
-  const bool large = __builtin_amdgcn_ballot_w64(most > kLargeScale) != 0, finite = __builtin_amdgcn_ballot_w64(most >= 0x7C00u) == 0;
-  __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, __builtin_amdgcn_readfirstlane(large && finite ? 1 : 0));
+  return __builtin_amdgcn_ballot_w64(most > kLargeScale) != 0 && __builtin_amdgcn_ballot_w64(most >= 0x7C00u) == 0;
+}
+__device__ __forceinline__ void SetSaturation(bool on) {
+  __builtin_amdgcn_sched_barrier(0);
+  if (on) __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, 1);
+  else __builtin_amdgcn_s_setreg((0 << 11) | (23 << 6) | 1, 0);
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // K's do not: a saturated product would be another score, and an infinite one a NaN. A tile with a large scale enters the
@@ -327,6 +333,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
     for (int j = 0; j < PPT; ++j) pgc[j] = pgn[j];
     load_pages(tile + step < tile1 ? tile + step : tile, pgn);
     const bool cut = (tile + 1) * kTile > n_keys;
+    bool saturates;
     int up = 0;  // this tile's scores come times 2^-up
     {  // scales to LDS; the V scales of masked keys become 0, which makes their V rows 0 whatever they hold
       uint32_t w[4] = {vsr.x, vsr.y, vsr.z, vsr.w};
@@ -341,7 +348,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
         *reinterpret_cast<uint4*>(&lds.k[lane * 8]) = ksr;
         *reinterpret_cast<uint4*>(&lds.v[lane * 8]) = uint4{w[0], w[1], w[2], w[3]};
       }
-      SetSaturation(uint4{w[0], w[1], w[2], w[3]});
+      saturates = Saturates(uint4{w[0], w[1], w[2], w[3]});
     }
     load_scales(pgn);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -391,6 +398,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
       Numerators<D>(st[i], tscale, m[i], l[i], o[i], pv[i]);
     }
     // ---- O^T
+    if (__builtin_expect(saturates, 0)) SetSaturation(true);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const h8v s0 = *reinterpret_cast<const h8v*>(&lds.v[b * kTile + 16 * jg]);
@@ -412,6 +420,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if (__builtin_expect(saturates, 0)) SetSaturation(false);
     __builtin_amdgcn_wave_barrier();  // (the scales in LDS are rewritten for the next tile)
   }
 }
