@@ -442,10 +442,11 @@ int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* pools, const
 /* ---- attention over a shared prefix ---------------------------------------------------------------------------------------
  * Decode attention for a batch whose sequences begin with prefixes they share, each prefix's keys read and decoded once for
  * all the query rows that see them. Sequences group_first[j] .. group_first[j + 1] - 1 form group j (device int32
- * [n_groups + 1], rising from 0 to n_seqs), and their page-table rows name the same pages for the prefix's first
- * 64 * floor(shared_len[j] / 64) tokens (device int32 [n_groups]; forks share a prefix's full pages): these are read
- * through the row of the group's first sequence, the rest of every sequence through its own row. A sequence
- * shorter than those tiles is read through its own row alone (max_tail_len has to cover it); one of length 0 gives zeros.
+ * [n_groups + 1], rising from 0 to n_seqs). Those of at least 64 * floor(shared_len[j] / 64) tokens (device int32 [n_groups]) have
+ * page-table rows that name the same pages for these tokens (forks share a prefix's full pages), which are read through
+ * the row of the first of them, and what follows through every sequence's own row. A shorter sequence, also an idle slot at the head
+ * of its group, is read through its own row alone, whatever that names (max_tail_len has to cover it); one of length 0 gives
+ * zeros.
  * Results are those of yahkv_decode_attend up to the order of the sums
  * (both within 2e-3 of exact arithmetic on the dequantized K / V; a 16-bit out adds its own rounding).
  *   q, gate    as yahkv_decode_attend

@@ -287,3 +287,33 @@ def test_nan_and_infinite_queries_give_nan_beside_large_scales(yahkv, torch_gpu,
     for s in range(4):
         for h in range(8):
             assert (torch.isnan(out[s, h]) if (s, h) in bad else torch.isfinite(out[s, h])).all(), (s, h)
+
+
+@pytest.mark.parametrize("leaders", [[0], [100], [0, 63, 191], [0] * 70, [5, 0] * 40])
+@pytest.mark.parametrize("bound", [0, 65536])
+def test_a_group_led_by_sequences_shorter_than_its_prefix(yahkv, torch_gpu, leaders, bound):
+    """Sequences that are shorter than the prefix's tiles (idle slots among them) are read through their own rows alone, also at
+    the head of a group: their rows name other pages than the prefix's."""
+    torch = torch_gpu
+    n_q, n_kv, hd, pt = 8, 2, 128, 32
+    groups = [(192, leaders + [250, 0, 300]), (0, [70]), (130, [5, 128, 200]), (256, [0, 9])]
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, 8, n_q, n_kv, hd, pt, groups, len(leaders) + sum(leaders), spare=4 * len(leaders) + 16)
+    rng = np.random.default_rng(3)
+    free = [p for p in range(g.n_pages) if p not in set(table.reshape(-1).tolist())]
+    at, n = 0, len(leaders)
+    for s in list(range(n)) + [n + 1, n + 4, len(lens) - 2, len(lens) - 1]:
+        need = max((lens[s] + pt - 1) // pt, 1)
+        table[s] = free[at]                                                # a page that holds nothing written
+        table[s, :need] = free[at:at + need]
+        at += need
+        if lens[s]:
+            oracle.append(host, table[s:s + 1], [0], None, *(to_bf16_f32(rng.standard_normal((1, lens[s], n_kv, hd))) for _ in range(2)))
+    dev.load(host.arrays())
+    a["table"] = torch.from_numpy(table).cuda()
+    if bound:
+        a.update(max_shared_len=bound, max_tail_len=40000)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), 0.1)
+    got = yahkv.decode_attend_shared(dev, q=q.half(), scale=0.1, **a)
+    check(torch, got, want, torch.float32)
+    for s, m in enumerate(lens):
+        assert m > 0 or not got[s].any()

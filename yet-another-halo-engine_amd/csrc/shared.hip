@@ -496,7 +496,9 @@ __device__ __forceinline__ void MergeWaves(const SharedArgs& a, SharedLds<D, RB>
 // A piece of a prefix against a block of ROWS of its group's rows, by workgroup. Those that read the same keys (the row
 // blocks of a piece) run on one XCD, side by side.
 struct PrefixPiece {
-  int group, h, piece, first, row0, n_rows, tile0, tile1;  // group -1: nothing; n_rows: rows from row0 on
+  // group -1: nothing; n_rows: rows from row0 on. The pages are read through the row of sequence `reader`, the group's first
+  // one that takes the prefix (KeysOf): the row of a shorter one, an idle slot's above all, need not name them.
+  int group, h, piece, first, reader, row0, n_rows, tile0, tile1;
   __device__ __forceinline__ size_t Row(const SharedArgs& a, int r) const {  // row r of the block among all (sequence, query head) rows
     const int G = a.g.group(), rr = row0 + min(r, n_rows - 1);
     return (size_t(first) + rr / G) * a.g.n_q + size_t(h) * G + rr % G;
@@ -507,13 +509,13 @@ __device__ __forceinline__ PrefixPiece FindPiece(const SharedArgs& a) {
   const int G = a.g.group(), H = a.g.n_kv, lane = threadIdx.x % 64;
   const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
   const int pair = xcd + 8 * (local / a.max_blocks), block = local % a.max_blocks;
-  PrefixPiece p{-1, pair % H, pair / H, 0, 0, 0, 0, 0};
+  PrefixPiece p{-1, pair % H, pair / H, 0, 0, 0, 0, 0, 0};
   if (pair >= H * a.n_split) return p;
-  int tiles = 0;
+  int tiles = 0, n_seqs = 0, first_len = 0;
   for (int j0 = 0, before = 0; j0 < a.n_groups; j0 += 64) {  // lane = group: which one row block `block` lies in
     const int j = min(j0 + lane, a.n_groups - 1);
     const int first = GroupFirst(a, j), rows = j0 + lane < a.n_groups ? max(GroupFirst(a, j + 1) - first, 0) * G : 0;
-    const int shared = GroupShared(a, j), n = (rows + ROWS - 1) / ROWS;
+    const int shared = GroupShared(a, j), n = (rows + ROWS - 1) / ROWS, len = a.seq_len[min(first, a.n_seqs - 1)];
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -525,7 +527,7 @@ __device__ __forceinline__ PrefixPiece FindPiece(const SharedArgs& a) {
       const int at = __builtin_ctzll(mine);
       auto its = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
       p.group = j0 + at, p.row0 = (block - before - its(incl - n)) * ROWS;
-      p.first = its(first), p.n_rows = its(rows) - p.row0, tiles = its(shared) / kTile;
+      p.first = its(first), n_seqs = its(rows) / G, p.n_rows = its(rows) - p.row0, tiles = its(shared) / kTile, first_len = its(len);
       break;
     }
     before += __builtin_amdgcn_readlane(incl, 63);
@@ -534,6 +536,20 @@ __device__ __forceinline__ PrefixPiece FindPiece(const SharedArgs& a) {
   const int per = PerPiece(tiles, a.n_split);
   p.tile0 = p.piece * per, p.tile1 = min(p.tile0 + per, tiles);
   if (p.tile0 >= p.tile1) p.group = -1;
+  if (p.group < 0) return p;
+  p.reader = p.first;
+  if (__builtin_expect(first_len < tiles * kTile, 0)) {
+    const int group = p.group;
+    p.group = -1;  // (if there is none, nobody reads the partials)
+    for (int m0 = 0; m0 < n_seqs; m0 += 64) {
+      const bool takes = m0 + lane < n_seqs && a.seq_len[p.first + min(m0 + lane, n_seqs - 1)] >= tiles * kTile;
+      const unsigned long long who = __ballot(takes);
+      if (who != 0) {
+        p.group = group, p.reader = p.first + m0 + __builtin_ctzll(who);
+        break;
+      }
+    }
+  }
   return p;
 }
 
@@ -572,7 +588,7 @@ __global__ __launch_bounds__(64 * kSharedWaves, RB * D <= 256 ? 2 : 1) void Shar
   queries.Request(a.q, a.q_dtype, row_of);
   float m[RB], l[RB];
   f4v o[RB][D / 16];
-  StreamKeys<FMT, D, PT, RB, TWO>(a, a.table + int64_t(pp.first) * a.stride, 0, pp.h, pp.tile0 + wave, kSharedWaves, pp.tile1,
+  StreamKeys<FMT, D, PT, RB, TWO>(a, a.table + int64_t(pp.reader) * a.stride, 0, pp.h, pp.tile0 + wave, kSharedWaves, pp.tile1,
                              pp.tile1 * kTile, queries, lds.scales[wave], m, l, o);
   // (rows of sequences shorter than the prefix leave partials that nobody reads)
   MergeWaves<D, RB>(a, lds, m, l, o, pp.n_rows, row_of, pp.piece);
