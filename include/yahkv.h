@@ -382,8 +382,8 @@ int yahkv_slot_unpack(const yahkv_geometry* g, const yahkv_pools* pools, const i
  * first_dim + 2 p + 1) in the INTERLEAVED one; the other dims pass through. With `normalise` every row first becomes
  * (x * rsqrt(sum x^2 / head_dim + eps)) * weight, all its dims.
  * Frequencies are held in turns as binary fractions, f_p / (2 pi) * 2^64: an integer product with the position, modulo
- * 2^64, is the angle's fraction of a turn without any loss however far the position, so angles are exact to f32's last
- * bits at every int32 position, also negative ones. */
+ * 2^64, is the angle's fraction of a turn without any loss however far the position. The table's entries are within 2^-63
+ * turns, so the angle of any int32 position, also a negative one, is within 2^-31 turns (3e-9 radians) of pos * f_p. */
 typedef enum yahkv_rotary_layout { YAHKV_ROTARY_HALF = 0, YAHKV_ROTARY_INTERLEAVED = 1 } yahkv_rotary_layout;
 typedef enum yahkv_rotary_scaling {
   YAHKV_ROTARY_PLAIN = 0,   /* f_p = theta^(-2 p / rotary_dim) */

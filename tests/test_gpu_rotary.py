@@ -12,7 +12,7 @@ import pytest
 
 import oracle
 from helpers import make_tables
-from test_host_serving import frequencies
+from test_host_serving import exact_turns, frequencies
 
 pytestmark = pytest.mark.gpu
 SPEC = dict(none=0, linear=1, ntk=2, yarn=3, bands=4)
@@ -69,6 +69,26 @@ def test_scalings_and_far_positions(yahkv, torch_gpu, layout, scaling):
         want = want_rows(x.cpu().numpy(), pos, 128, layout, scaling)
         tol = (2.4e-6 * 2.6 + 2.6 * spread) * np.abs(want).max(-1, keepdims=True)
         assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.parametrize("scaling", sorted(SPEC))
+@pytest.mark.parametrize("theta", [1e4, 1e7])
+def test_angles_of_far_positions(yahkv, torch_gpu, theta, scaling):
+    """Pairs (1, 0) become the cosine and sine themselves: against frequencies of 60 digits, so that a far position shows what the
+    table lacks. Tolerance: 4 u = 2.4e-7 of a sine (above), and of the angle 2^-63 turns times the position (the table, tested on
+    the host) and 2^-32 turns (the bits of the fraction that the sine drops): 2^-32 + 2^-32 turns, 2.9e-9 radians."""
+    from fractions import Fraction
+    torch = torch_gpu
+    pos = [0, 1, -1, 4095, 123456, 10 ** 6 + 3, 2 ** 28 + 1, 2 ** 31 - 1, -2 ** 31, -2 ** 31 + 12345]
+    low, high = (1.0, 4.0) if scaling == "bands" else (1.0, 32.0)
+    f = [Fraction(x) for x in exact_turns(64, SPEC[scaling], theta, 8.0, 4096.0, low, high)]
+    a = np.array([[float(p * x % 1) for x in f] for p in pos]) * 2 * np.pi
+    q = torch.zeros(len(pos), 1, 1, 64, device="cuda")
+    q[..., :32] = 1.0
+    r = make(yahkv, 64, "half", scaling, theta=theta, magnitude=1.0)
+    y, _ = yahkv.rotary_rows(r, torch.tensor(pos, dtype=torch.int32, device="cuda")[:, None], q)
+    y = y.double().cpu().numpy()[:, 0, 0]
+    assert np.abs(y[:, :32] - np.cos(a)).max() <= 2.4e-7 + 2.9e-9 and np.abs(y[:, 32:] - np.sin(a)).max() <= 2.4e-7 + 2.9e-9
 
 
 @pytest.mark.parametrize("d,dim,first", [(8, 8, 0), (40, 16, 8), (64, 32, 32), (80, 80, 0), (96, 64, 4), (128, 128, 0), (192, 64, 128),

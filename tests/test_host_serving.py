@@ -62,6 +62,47 @@ def test_rotary_table_keeps_far_positions_exact(yahkv):
             assert Fraction(pos * int(f) % 2 ** 64, 2 ** 64) == exact
 
 
+def exact_turns(dim, scaling, theta, factor, length, low, high):
+    """The frequencies of include/yahkv.h in turns, to 60 decimal digits."""
+    from decimal import Decimal as D, ROUND_CEILING, ROUND_FLOOR, localcontext
+    with localcontext() as c:
+        c.prec = 60
+        pi2 = D("6.28318530717958647692528676655900576839433879875021164194988918461563281257")
+        theta, factor, length, low, high = D(theta), D(factor), D(length), D(low), D(high)
+        if scaling == 2:
+            theta *= (factor.ln() * dim / (dim - 2)).exp()
+        edge = lambda n: dim * (length / (n * pi2)).ln() / (2 * theta.ln())
+        a = max(edge(high).to_integral_value(ROUND_FLOOR), D(0))
+        b = min(edge(low).to_integral_value(ROUND_CEILING), D(dim - 1))
+        got = []
+        for p in range(dim // 2):
+            f = (theta.ln() * -2 * p / dim).exp()
+            if scaling == 1:
+                f /= factor
+            elif scaling == 3:
+                x = min(D(1), max(D(0), (p - a) / max(b - a, D(0.001))))
+                f = f / factor * x + f * (1 - x)
+            elif scaling == 4:
+                x = min(D(1), max(D(0), (length * f / pi2 - low) / (high - low)))
+                f = f / factor * (1 - x) + f * x
+            got.append(f / pi2)
+        return got
+
+
+@pytest.mark.parametrize("scaling", range(5))
+@pytest.mark.parametrize("dim,theta", [(8, 1e4), (64, 1e4), (64, 1e7), (72, 1e6), (128, 5e5), (256, 1e7), (512, 1.5)])
+def test_rotary_table_to_its_last_bits(yahkv, dim, theta, scaling):
+    """Every entry within two of its units, 2^-63 turns: half of one is its own rounding, and the operations before it, in 64 bits
+    of significand, err by a few 2^-64 of a frequency that is 2^61.4 units at most (powers one step of 2^-63, its exponent,
+    quotients and products half of one each, and the ramp of the banded rules up to twice as many: 8 x 2^-64 x 2^61.4 = 1.4)."""
+    from decimal import Decimal as D
+    low, high = (1.0, 4.0) if scaling == 4 else (1.0, 32.0)
+    rc, turns, _ = table(yahkv, dim, scaling, theta, 8.0, 32768.0, low, high)
+    assert rc == 0
+    off = [abs(D(int(t)) - w * 2 ** 64) for t, w in zip(turns, exact_turns(dim, scaling, theta, 8.0, 32768.0, low, high))]
+    assert max(off) <= 2, float(max(off))
+
+
 @pytest.mark.parametrize("change", [dict(dim=4), dict(dim=0), dict(dim=-8), dict(dim=12), dict(theta=1.0), dict(theta=float("nan")),
                                     dict(theta=float("inf")), dict(scaling=5), dict(scaling=-1), dict(scaling=1, factor=0.5),
                                     dict(scaling=1, factor=float("nan")), dict(scaling=3, length=0.0), dict(scaling=4, low=0.0),

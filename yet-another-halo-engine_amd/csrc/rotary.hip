@@ -156,7 +156,6 @@ using namespace yahkv;
 extern "C" int yahkv_rotary_table(const yahkv_rotary_spec* spec, uint64_t* turns, float* magnitude) {
   if (spec == nullptr || turns == nullptr || magnitude == nullptr) return YAHKV_ERR_ARG;
   const int r = spec->rotary_dim, half = r / 2;
-  const double pi2 = 6.283185307179586476925286766559;
   if (r < 8 || r % 8 != 0 || !(spec->theta > 1.0) || !std::isfinite(spec->theta)) return YAHKV_ERR_ARG;
   if (spec->scaling < YAHKV_ROTARY_PLAIN || spec->scaling > YAHKV_ROTARY_BANDS) return YAHKV_ERR_ARG;
   const bool bands = spec->scaling == YAHKV_ROTARY_YARN || spec->scaling == YAHKV_ROTARY_BANDS;
@@ -165,26 +164,30 @@ extern "C" int yahkv_rotary_table(const yahkv_rotary_spec* spec, uint64_t* turns
   if (bands && (!(spec->original_len > 0.0) || !std::isfinite(spec->original_len) || !(spec->low > 0.0) ||
                 !(spec->high > spec->low) || !std::isfinite(spec->high)))
     return YAHKV_ERR_ARG;
-  double theta = spec->theta;
-  if (spec->scaling == YAHKV_ROTARY_NTK) theta *= std::pow(f, double(r) / (r - 2));
+  // In 64 bits of significand: an entry's unit is 2^-64 of a turn, and a double's last bit of the fast pairs is 2^8 of them,
+  // 3e-7 radians at position 2^31. The entries are within 2^-63 turns.
+  typedef long double real;  // (x86-64's)
+  const real pi2 = 6.283185307179586476925286766559005768L, factor = f, length = spec->original_len, low = spec->low, high = spec->high;
+  real theta = spec->theta;
+  if (spec->scaling == YAHKV_ROTARY_NTK) theta *= std::pow(factor, real(r) / (r - 2));
   // YaRN: the pairs that make `high` and `low` turns within the original context bound the ramp, in whole pairs
-  double ramp0 = 0.0, ramp1 = 1.0;
+  real ramp0 = 0, ramp1 = 1;
   if (spec->scaling == YAHKV_ROTARY_YARN) {
-    auto pair_of = [&](double n) { return r * std::log(spec->original_len / (n * pi2)) / (2.0 * std::log(theta)); };
-    ramp0 = std::fmax(std::floor(pair_of(spec->high)), 0.0), ramp1 = std::fmin(std::ceil(pair_of(spec->low)), r - 1.0);
+    auto pair_of = [&](real n) { return r * std::log(length / (n * pi2)) / (2 * std::log(theta)); };
+    ramp0 = std::fmax(std::floor(pair_of(high)), real(0)), ramp1 = std::fmin(std::ceil(pair_of(low)), real(r - 1));
   }
   for (int p = 0; p < half; ++p) {
-    const double inv = std::pow(theta, -2.0 * p / r);
-    double w = inv;
-    if (spec->scaling == YAHKV_ROTARY_LINEAR) w = inv / f;
+    const real inv = std::pow(theta, -2 * real(p) / r);
+    real w = inv;
+    if (spec->scaling == YAHKV_ROTARY_LINEAR) w = inv / factor;
     if (spec->scaling == YAHKV_ROTARY_YARN) {
-      const double x = std::fmin(std::fmax((p - ramp0) / std::fmax(ramp1 - ramp0, 0.001), 0.0), 1.0);
-      w = inv / f * x + inv * (1.0 - x);
+      const real x = std::fmin(std::fmax((p - ramp0) / std::fmax(ramp1 - ramp0, real(0.001)), real(0)), real(1));
+      w = inv / factor * x + inv * (1 - x);
     }
     if (spec->scaling == YAHKV_ROTARY_BANDS) {
-      const double n = spec->original_len * inv / pi2;  // turns within the original context
-      const double x = std::fmin(std::fmax((n - spec->low) / (spec->high - spec->low), 0.0), 1.0);
-      w = inv / f * (1.0 - x) + inv * x;
+      const real n = length * inv / pi2;  // turns within the original context
+      const real x = std::fmin(std::fmax((n - low) / (high - low), real(0)), real(1));
+      w = inv / factor * (1 - x) + inv * x;
     }
     turns[p] = static_cast<uint64_t>(std::rint(std::ldexp(w / pi2, 64)));  // w <= 1: below 2^62
   }

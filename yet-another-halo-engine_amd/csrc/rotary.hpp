@@ -21,7 +21,7 @@ struct RowsArgs {
 };
 
 // cos and sin of the angle pos * f, f in turns as a 0.64 binary fraction: the product modulo 2^64 is the angle's exact
-// fraction of a turn (f itself is rounded to 2^-65 turns: at position 2^31 that is 2^-34 turns). Its top 32 bits split
+// fraction of a turn (yahkv_rotary_table's f is within 2^-63 turns: at position 2^31 that is 2^-32 turns). Its top 32 bits split
 // into a quarter turn and a remainder x of at most an eighth of a turn either way, which f32 holds to 2^-24 relative; on
 // |x| <= pi / 4 the Taylor sums up to x^9 and x^8 are short of sine and cosine by x^11 / 11! < 2^-28 and x^10 / 10! < 2^-25.
 __device__ __forceinline__ void TurnCosSin(int pos, uint64_t turns, float* c, float* s) {
