@@ -302,3 +302,23 @@ def test_output_types_are_refused(yahkv):
     with pytest.raises(yahkv.YahkvError):
         yahkv._out(torch.zeros(1, 8, 128, dtype=torch.int32), q, None, torch.float32)
     assert yahkv._out(None, q.transpose(1, 2), torch.bfloat16, torch.float32).is_contiguous()
+
+
+def test_rotary_outputs_of_another_type_than_asked_for_are_refused(yahkv):
+    """(A call that passes every look at its tensors is refused for their device here.)"""
+    import torch
+    r = yahkv.Rotary(64, 1e4, device="cpu")
+    pos, x = torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, 1, 2, 128)
+    half, same = x.half(), torch.empty_like(x)
+    for a in (dict(q_out=half, out_dtype=torch.float32), dict(k=x, q_out=same, k_out=half, out_dtype=torch.float32)):
+        with pytest.raises(yahkv.YahkvError, match="another type"):
+            yahkv.rotary_rows(r, pos, x, **a)
+    for a in (dict(q_out=half), dict(q_out=half, out_dtype=torch.float16), dict(k=x, q_out=half, out_dtype=torch.float32)):
+        with pytest.raises(yahkv.YahkvError, match="on a GPU"):
+            yahkv.rotary_rows(r, pos, x, **a)
+    g = yahkv.geometry(8, 4, 2, 128, 16, 4)
+    dev, i, q = yahkv.DevicePools(g, device="cpu"), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 1, 4, 128)
+    for a, why in ((dict(q_out=q.half(), q_out_dtype=torch.float32), "another type"), (dict(q_out=q.half()), "on a GPU"),
+                   (dict(q_out=q.half(), q_out_dtype=torch.float16), "on a GPU"), (dict(q_out_dtype=torch.float16), "on a GPU")):
+        with pytest.raises(yahkv.YahkvError, match=why):
+            yahkv.rotary_append(dev, torch.zeros(3, 1, dtype=torch.int32), i, r, x, x, q, **a)

@@ -785,7 +785,8 @@ def _ref(s):
 def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_dtype=None):
     """Rotates q and / or k, [n_seqs][n_new][heads][D] tensors at any strides of whole 16 bytes (slices of a fused projection),
     token t of sequence s by positions[s][t] (int32). Returns (q_out, k_out), new contiguous tensors of out_dtype (the rows'
-    own by default) where none are given; q_out may be q itself. None for rows that were not given."""
+    own by default) where none are given; q_out may be q itself. out_dtype without a new tensor to be of it has to be the given
+    ones' type. None for rows that were not given."""
     first = q if q is not None else k
     if first is None or first.dim() != 4:
         _refuse("rotary_rows: q or k [n_seqs][n_new][heads][D]")
@@ -795,7 +796,7 @@ def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_d
     rotary.check_head(d)
     if rotary.turns.device != dev:
         _refuse("rotary_rows: the frequency table is on another device")
-    refs, outs = [], []
+    refs, outs, wrong, new = [], [], False, False
     for x, out in ((q, q_out), (k, k_out)):
         if x is None:
             _need(out is None, "rotary_rows: an output without its rows")
@@ -810,12 +811,16 @@ def rotary_rows(rotary, positions, q=None, k=None, q_out=None, k_out=None, out_d
             if dtype not in _DTYPES:
                 _refuse(f"rotary_rows: out_dtype {dtype}")
             out, dst = _new_rows(x, dtype)
+            new = True
         else:
             if out.shape != shape or out.device != dev:
                 _refuse("rotary_rows: out has the rows' shape")
             dst = _rows(out, "rotary_rows")
+            wrong = wrong or out_dtype not in (None, out.dtype)
         refs += (C.byref(src), C.byref(dst))
         outs.append(out)
+    if wrong and not new:
+        _refuse(f"rotary_rows: out_dtype {out_dtype}, and an output of another type")
     _run_on(dev, lambda st: lib.yahkv_rotary_apply(C.byref(rotary.struct), d, positions.data_ptr(), n_seqs, n_new, *refs, st),
             "rotary_apply")
     return tuple(outs)
@@ -849,6 +854,7 @@ def rotary_append(pools, table, start_pos, rotary, k, v, q=None, positions=None,
             q_out, qd = _new_rows(q, q_out_dtype or torch.float32)
         else:
             _need(q_out.shape == q.shape and q_out.device == dev, "rotary_append: q_out has q's shape")
+            _need(q_out_dtype in (None, q_out.dtype), f"rotary_append: q_out_dtype {q_out_dtype}, and a q_out of another type")
             qd = _rows(q_out, "q_out")
     _need(q is not None or q_out is None, "rotary_append: q_out without q")
     _need(k_out is None or (k_out.dtype == torch.float32 and k_out.is_contiguous() and k_out.shape == k.shape and
