@@ -322,3 +322,13 @@ def test_rotary_outputs_of_another_type_than_asked_for_are_refused(yahkv):
                    (dict(q_out=q.half(), q_out_dtype=torch.float16), "on a GPU"), (dict(q_out_dtype=torch.float16), "on a GPU")):
         with pytest.raises(yahkv.YahkvError, match=why):
             yahkv.rotary_append(dev, torch.zeros(3, 1, dtype=torch.int32), i, r, x, x, q, **a)
+
+
+@pytest.mark.parametrize("name", ["ks", "vq", "vs"])
+def test_pools_on_two_devices_are_refused(yahkv, name):
+    g = yahkv.geometry(8, 8, 2, 128, 16, 4)
+    t = yahkv.DevicePools(g, device="cpu")
+    a = dict(kq=t.kq, ks=t.ks, vq=t.vq, vs=t.vs)
+    assert yahkv.DevicePools.of(g, **a).vs.data_ptr() == t.vs.data_ptr()
+    with pytest.raises(yahkv.YahkvError, match="device"):
+        yahkv.DevicePools.of(g, **dict(a, **{name: a[name].to("meta")}))

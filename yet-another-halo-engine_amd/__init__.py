@@ -357,12 +357,14 @@ class DevicePools:
 
     @classmethod
     def of(cls, g, kq, ks, vq, vs):
-        """Pools over buffers the caller has: contiguous tensors of any type and shape, as long as the geometry needs."""
+        """Pools over buffers the caller has: contiguous tensors of any type and shape on one device, as long as the
+        geometry needs."""
         import torch
         self = cls.__new__(cls)
         self.geom = g
         for name, t in (("kq", kq), ("ks", ks), ("vq", vq), ("vs", vs)):
             _need(t.is_contiguous(), f"pools: {name} is not contiguous")
+            _need(t.device == kq.device, f"pools: {name} is on another device than kq")
             setattr(self, name, t.view(-1).view(torch.uint8))
         return self
 
