@@ -73,6 +73,33 @@ def test_weights(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, lens):
         assert np.array_equal(base[s, :, m:].double().cpu().numpy(), b64[s, :, m:])
 
 
+@pytest.mark.parametrize("fmt,n_q,n_kv,hd,pt", [
+    (8, 24, 4, 256, 64), (8, 8, 1, 256, 32), (8, 6, 3, 256, 16), (8, 32, 8, 128, 64), (8, 10, 5, 128, 32), (8, 4, 2, 128, 16),
+    (4, 8, 1, 256, 64), (4, 24, 4, 256, 32), (4, 16, 8, 256, 16), (4, 6, 3, 128, 64), (4, 3, 1, 128, 32), (4, 32, 8, 128, 16)])
+def test_weights_of_a_large_batch(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt):
+    """The form for batches of more tiles than waves hold (a partial per wave, the line cut by tile where the kv heads divide
+    eight): the host's bound alone asks for it, the lengths stay short."""
+    torch = torch_gpu
+    lens = [700, 1, 0, 64, 65, 333, 2000, 17, 0, 130]
+    g, table, host, dev, rng = setup(yahkv, torch, fmt, n_q, n_kv, hd, pt, lens, seed=hd + pt + n_kv, fill=0x7F)
+    n, T, bound, scale = len(lens), max(lens), 70001, hd ** -0.5
+    q = torch.from_numpy(rng.standard_normal((n, n_q, hd)).astype(np.float32)).cuda().to(torch.bfloat16)
+    t_table, t_len = torch.from_numpy(table).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want, rel = exact_weights(g, table, host, lens, q.double().cpu().numpy(), scale)
+    out_want = closed(g, table, host, lens, q.double().cpu().numpy(), scale)
+    base = torch.rand(n, n_kv, bound + 2, device="cuda") * 3
+    b64 = base[:, :, :T].double().cpu().numpy()
+    w = base.clone()
+    out = yahkv.decode_attend_weights(dev, t_table, t_len, bound, q, scale, w, weights_in=w, decay=0.5)
+    check(torch, out, out_want, torch.float32)
+    got = w[:, :, :T].double().cpu().numpy()
+    for s, m in enumerate(lens):
+        total = 0.5 * b64[s, :, :m] + want[s, :, :m]
+        assert np.all(np.abs(got[s, :, :m] - total) <= want[s, :, :m] * rel[s][:, None] + total * 2 * U), s
+        assert torch.equal(w[s, :, m:], base[s, :, m:])                        # behind the length: left alone
+        assert m > 0 or not out[s].any()
+
+
 def test_weights_from_a_graph(yahkv, torch_gpu):
     torch = torch_gpu
     lens = [700, 64, 0, 333]
