@@ -222,17 +222,18 @@ __global__ __launch_bounds__(64 * kRopeWaves) void AppendRows(const RopeArgs a) 
 constexpr int kPageWaves = 4;
 constexpr int kPageAppendMin = 8;  // tokens per sequence from which a call is treated as a chunk
 // SRC: the source rows' type, known when compiling (as a run-time value it put a three-way branch around every
-// row's conversion).
+// row's conversion). D: the head dim (as a run-time value whether a wavefront's sets are one or two made every token's address the
+// vector unit's: 8 x 2048 tokens of 4 heads of 256 dims 31.1 us, 29.9 as a constant).
 // TURN: yahkv_rotary_append's chunks: the K rows of a wave's four tokens are normalised and turned before they are quantized.
 // Their cosines and sines are worked out by the wave into LDS, again for every kv head's workgroup (a twentieth of the
 // kernel's instructions; a table for all heads would need memory and a launch of its own).
-template <int FMT, int SRC, bool TURN>
+template <int FMT, int SRC, bool TURN, int D>
 __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a) {
 #pragma clang fp contract(off)
   const Geom g = a.g;
-  const int NB = g.nb(), H = g.n_kv, PT = g.pt, D = g.hd;
-  constexpr int KB = FMT == 8 ? 32 : 16;                 // bytes of K codes per token and block
-  const int v_rows = FMT == 8 ? D : NB * 16;             // byte rows of the V image, PT bytes each
+  const int H = g.n_kv, PT = g.pt;
+  constexpr int NB = D / 32, KB = FMT == 8 ? 32 : 16;    // blocks, bytes of K codes per token and block
+  constexpr int v_rows = FMT == 8 ? D : NB * 16;             // byte rows of the V image, PT bytes each
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, h = blockIdx.y, s = blockIdx.z;
   const int nv = a.n_valid != nullptr ? min(max(a.n_valid[s], 0), a.n_new) : a.n_new;
   if (nv <= 0) return;
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(64 * kPageWaves) void AppendPages(const RopeArgs a)
   __shared__ __align__(16) uint16_t lks[64 * 8], lvs[8 * 64];      // and of the scale regions
   // A row lies across D / 4 lanes, so that at 128 dims a wavefront has two sets of four tokens side by side (5 x 1037 tokens of 8
   // heads, pages of 32: 14.4 us, turned 24.4; with half the lanes idle 18.9 and 31.6).
-  const int row_lanes = D / 4, sets = 64 / row_lanes, set = lane / row_lanes, rl = lane % row_lanes;
+  constexpr int row_lanes = D / 4, sets = 64 / row_lanes;
+  const int set = lane / row_lanes, rl = lane % row_lanes;
   const int d0 = 4 * rl, b = rl / 8, lb = rl % 8;
   // A set of lanes takes four consecutive tokens at a time (their rows in flight together): a lane then holds, for each
   // of its four dims, the codes of four neighbouring tokens, which is one dword of the V image instead of four bytes.
@@ -493,20 +495,25 @@ int CheckAppend(const yahkv_geometry* g, const yahkv_pools* pools, const int32_t
 namespace {
 // AppendRows for the pools' format and the source rows' type (the kernel is compiled for each pair)
 // AppendPages likewise: one workgroup per (page the chunk touches, kv head, sequence)
+template <bool TURN, int D>
+void LaunchPagesOf(int32_t format, int32_t src_dtype, dim3 grid, hipStream_t st, const RopeArgs& a) {
+  const dim3 block(64 * kPageWaves);
+  if (format == YAHKV_Q8_0) {
+    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<8, YAHKV_F32, TURN, D>), grid, block, 0, st, a);
+    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<8, YAHKV_F16, TURN, D>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((AppendPages<8, YAHKV_BF16, TURN, D>), grid, block, 0, st, a);
+  } else {
+    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<4, YAHKV_F32, TURN, D>), grid, block, 0, st, a);
+    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<4, YAHKV_F16, TURN, D>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((AppendPages<4, YAHKV_BF16, TURN, D>), grid, block, 0, st, a);
+  }
+}
 template <bool TURN>
 void LaunchPages(int32_t format, int32_t src_dtype, int32_t n_seqs, int32_t n_new, hipStream_t st, const RopeArgs& a) {
   const dim3 grid(static_cast<unsigned>((n_new + a.g.pt - 2) / a.g.pt + 1), static_cast<unsigned>(a.g.n_kv),
                   static_cast<unsigned>(n_seqs));
-  const dim3 block(64 * kPageWaves);
-  if (format == YAHKV_Q8_0) {
-    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<8, YAHKV_F32, TURN>), grid, block, 0, st, a);
-    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<8, YAHKV_F16, TURN>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((AppendPages<8, YAHKV_BF16, TURN>), grid, block, 0, st, a);
-  } else {
-    if (src_dtype == YAHKV_F32) hipLaunchKernelGGL((AppendPages<4, YAHKV_F32, TURN>), grid, block, 0, st, a);
-    else if (src_dtype == YAHKV_F16) hipLaunchKernelGGL((AppendPages<4, YAHKV_F16, TURN>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((AppendPages<4, YAHKV_BF16, TURN>), grid, block, 0, st, a);
-  }
+  if (a.g.hd == 256) LaunchPagesOf<TURN, 256>(format, src_dtype, grid, st, a);
+  else LaunchPagesOf<TURN, 128>(format, src_dtype, grid, st, a);
 }
 template <int ROPE, int FLIGHT = kRowsInFlight>
 void LaunchRows(int32_t format, int32_t src_dtype, dim3 grid, hipStream_t st, const RopeArgs& a) {
