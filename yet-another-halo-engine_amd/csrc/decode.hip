@@ -1149,7 +1149,8 @@ constexpr int kReduceThreads = 256;  // also the number of partial slots weighed
 constexpr int kReduceThreadsWide = 512;  // ... where a pair has more than that many places for partials
 constexpr int kReduceDepth = 4;      // partials a group loads together
 constexpr int kReduceMinDims = 32;   // fewest dims of a head one workgroup sums
-template <int RT>
+// WEIGH: yahkv_decode_attend_weights' form: out of any type, and every row's maximum and sum.
+template <int RT, bool WEIGH>
 __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const StepRows rows) {
   const Geom g = a.g;
   const int G = g.group(), H = g.n_kv, D = g.hd;
@@ -1158,6 +1159,10 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
   // this workgroup's dims are [d0, d0 + DZ); the launch's z extent divides a head_dim of 128 or 256: a power of two
   const int DZ = D >> __builtin_ctz(gridDim.z), d0 = blockIdx.z * DZ;
   const size_t o = (size_t(s) * g.n_q + hq) * D + d0;
+  auto store = [&](size_t i, float v) {
+    if constexpr (WEIGH) Store1(a.out, i, a.out_dtype, v);
+    else a.out[i] = v;
+  };
   const int ts = TilesOf(a, s);
   // the step form: a sequence with a new token has it stored, and (but for the case StepSeesNewToken describes) attended to
   const bool stores_new = rows.k != nullptr && a.seq_len[s] >= 1;
@@ -1186,7 +1191,7 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
   if (p0 + t < p1) first_ml = *reinterpret_cast<const float2*>(&a.ml[((p0 + t) * G + gi) * 2]);
   if (stores_new && t < 128) StepToken(a, rows, s, h, hq, t / 64, t % 64, gi == 0 && blockIdx.z == 0, &new_score, new_v);
   if (ts <= 0 && !has_new) {  // nothing to attend to
-    for (int d = t; d < DZ; d += RT) Store1(a.out, o + d, a.out_dtype, 0.0f);
+    for (int d = t; d < DZ; d += RT) store(o + d, 0.0f);
     return;
   }
   constexpr int NW = RT / 64;
@@ -1257,10 +1262,10 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
     }
     v /= lt;
     if (a.gate != nullptr) v *= 1.0f / (1.0f + __expf(-a.gate[o + d]));
-    Store1(a.out, o + d, a.out_dtype, v);
-    if (a.row_ml != nullptr && d == 0 && d0 == 0) {
+    store(o + d, v);
+    if constexpr (WEIGH) {
       float* ml = a.row_ml + (size_t(s) * g.n_q + hq) * 2;
-      ml[0] = M, ml[1] = lt;
+      if (d == 0 && d0 == 0) ml[0] = M, ml[1] = lt;
     }
   }
 }
@@ -1349,10 +1354,15 @@ int LaunchReduce(const DecodeArgs& a, const StepRows& rows, const yahkv_decode_o
   // (a small batch cut into many chunks: a pair's places for partials, eight per chunk its tiles lie in, are weighed in
   // one sweep of a wider workgroup instead of two)
   const int64_t places = int64_t(a.n_chunks) * a.wpc / std::max<int64_t>(int64_t(a.n_seqs) * a.g.n_kv, 1) + a.wpc;
-  if (a.wg_partials && places > kReduceThreads)
-    hipLaunchKernelGGL(DattnReduce<kReduceThreadsWide>, dim3(a.g.n_q, a.n_seqs, split), dim3(kReduceThreadsWide), 0, st, a, rows);
-  else
-    hipLaunchKernelGGL(DattnReduce<kReduceThreads>, dim3(a.g.n_q, a.n_seqs, split), dim3(kReduceThreads), 0, st, a, rows);
+  const bool wide = a.wg_partials && places > kReduceThreads;
+  const dim3 grid(a.g.n_q, a.n_seqs, split), block(wide ? kReduceThreadsWide : kReduceThreads);
+  if (a.row_ml != nullptr) {
+    if (wide) hipLaunchKernelGGL((DattnReduce<kReduceThreadsWide, true>), grid, block, 0, st, a, rows);
+    else hipLaunchKernelGGL((DattnReduce<kReduceThreads, true>), grid, block, 0, st, a, rows);
+  } else {
+    if (wide) hipLaunchKernelGGL((DattnReduce<kReduceThreadsWide, false>), grid, block, 0, st, a, rows);
+    else hipLaunchKernelGGL((DattnReduce<kReduceThreads, false>), grid, block, 0, st, a, rows);
+  }
   return LaunchStatus();
 }
 
