@@ -244,6 +244,30 @@ def test_chunk_without_rotated_rows_leaves_the_same_pools(yahkv, torch_gpu, fmt,
             assert torch.equal(getattr(a, name), getattr(b, name)), name
 
 
+@pytest.mark.parametrize("n,new,pt", [(1, 130, 16), (2, 257, 32), (1, 300, 16)])
+def test_long_chunk_of_few_tokens_with_rotated_rows(yahkv, torch_gpu, n, new, pt):
+    """Chunks long enough to be dealt to the XCDs by pages and short enough for several workgroups a token."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda").manual_seed(new)
+    pages = new // pt + 2
+    g = yahkv.geometry(8, 8, 2, 128, pt, n * pages)
+    table = torch.randperm(n * pages, generator=gen, device="cuda").to(torch.int32).view(n, pages)
+    start = torch.tensor([5, 0][:n], dtype=torch.int32, device="cuda")
+    pos = torch.randint(0, 100000, (n, new), generator=gen, device="cuda", dtype=torch.int32)
+    x = torch.randn(n, new, 12, 128, generator=gen, device="cuda").half()
+    q, k, v = x[:, :, :8], x[:, :, 8:10], x[:, :, 10:]
+    r = make(yahkv, 64, "interleaved", "ntk", first_dim=32, normalise=True)
+    a, b = yahkv.DevicePools(g, fill=9), yahkv.DevicePools(g, fill=9)
+    k_out = torch.full(k.shape, float("nan"), device="cuda")
+    qa = yahkv.rotary_append(a, table, start, r, k, v, q, positions=pos, k_out=k_out)
+    qb = yahkv.rotary_append(b, table, start, r, k, v, q, positions=pos)
+    assert torch.equal(qa, qb)
+    for name in ("kq", "ks", "vq", "vs"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+    want = want_rows(k.double().cpu().numpy(), pos.cpu().numpy(), 64, "interleaved", "ntk", 32, normalise=True)
+    close(torch, k_out, want, torch.float32)
+
+
 def test_append_without_queries_or_norm_equals_rotate_then_append(yahkv, torch_gpu):
     torch = torch_gpu
     rng = np.random.default_rng(4)
