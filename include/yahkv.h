@@ -442,13 +442,17 @@ int yahkv_rotary_append(const yahkv_geometry* g, const yahkv_pools* pools, const
 /* ---- attention over a shared prefix ---------------------------------------------------------------------------------------
  * Decode attention for a batch whose sequences begin with prefixes they share, each prefix's keys read and decoded once for
  * all the query rows that see them. Sequences group_first[j] .. group_first[j + 1] - 1 form group j (device int32
- * [n_groups + 1], rising from 0 to n_seqs). Those of at least 64 * floor(shared_len[j] / 64) tokens (device int32 [n_groups]) have
- * page-table rows that name the same pages for these tokens (forks share a prefix's full pages), which are read through
- * the row of the first of them, and what follows through every sequence's own row. A shorter sequence, also an idle slot at the head
- * of its group, is read through its own row alone, whatever that names (max_tail_len has to cover it); one of length 0 gives
- * zeros.
- * Results are those of yahkv_decode_attend up to the order of the sums
- * (both within 2e-3 of exact arithmetic on the dequantized K / V; a 16-bit out adds its own rounding).
+ * [n_groups + 1], rising from 0 to n_seqs). Those of at least 64 * floor(shared_len[j] / 64) tokens (device int32
+ * [n_groups]) have page-table rows that name the same pages for these tokens (forks share a prefix's full pages): they are
+ * read through the row of the first of them, and what follows through every sequence's own row. A shorter sequence, also
+ * an idle slot at the head of its group, is read through its own row alone, whatever that names (max_tail_len has to cover
+ * it); one of length 0 gives zeros.
+ * Results are those of yahkv_decode_attend but for one rounding and the order of the sums: a K value d * code is rounded to f16
+ * here, as in the prefill, where yahkv_decode_attend takes the codes exactly and the scale in f32. Both are within 2e-3 (max
+ * |error| / max |value|) of exact arithmetic on the dequantized K / V; in the 2-norm an f32 out is 4.9e-4 off here and
+ * 2.2e-4 there (q8_0, scores of a standard deviation of two; 3.6e-4 and 2.6e-4 with one). A 16-bit out adds its own
+ * rounding. K values beyond +-65504 score as any others; finite V values beyond it saturate (among 64 keys that also have a V
+ * scale that is not finite they become infinite). NaN and infinities in a query give NaN, as there.
  *   q, gate    as yahkv_decode_attend
  *   out        [n_seqs][n_q_heads][D] of out_dtype (F32, F16 or BF16), 16-byte aligned
  *   max_shared_len, max_tail_len  host bounds: of shared_len[] (a longer prefix is cut to the bound and the rest counts as

@@ -263,7 +263,9 @@ __global__ __launch_bounds__(kCompactThreads) void EvictCompact(const CompactArg
   __syncthreads();
   const int dst_page = ClampPage(a.dst_table[static_cast<int64_t>(s) * a.dst_stride + page_i], g.n_pages);
   const size_t dph = static_cast<size_t>(dst_page) * H + h;
-  // K, asked for before V and stored after V's first loads are out: codes 16 bytes at a time, scales four blocks at a time
+  // K, asked for before V and stored after V's first loads are asked for: codes 16 bytes at a time, scales four blocks at a
+  // time. (Where a thread has two pieces or more the compiler keeps them in scratch memory on the way, and reading them back
+  // waits for V's first loads as well.)
   constexpr int KP = NB * PT * (KB / 16), KN = (KP + kCompactThreads - 1) / kCompactThreads;
   uint4 kc[KN];
   auto k_place = [&](int u, int* t) -> int {  // offset of piece u behind its token's place, pieces of a block by token

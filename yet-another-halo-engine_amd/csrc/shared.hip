@@ -16,13 +16,17 @@
 // keys of one dim (q4_0: of two). Row i of key tile kt is key 16 (i / 4) + 4 kt + i % 4: then the scores that lane group jg
 // holds after the four key tiles are those of keys 16 jg .. 16 jg + 15, the ones its V load has. P never leaves its lane.
 // A register is asked for again (for the wave's next tile) as soon as its codes are decoded, so a load has about a tile's
-// time to arrive, without a barrier anywhere in the loop. Decoding is packed f16 arithmetic, perm, add, multiply for two
+// time to arrive, without a barrier anywhere in the loop. (Not with 16-token pages: a tile's four page numbers, picked by
+// lane, lie in scratch memory there, and the waits for them are waits for every load that is out, two or three times a
+// tile.) Decoding is packed f16 arithmetic, perm, add, multiply for two
 // values, the product d * code rounded once; beyond the f16 range V's saturates (Saturates), K's takes a power of two
 // (ShrinkLargeKeys).
 // Roundings to f16 (11 bits): queries given as f32, K, V and the numerators, each once; products and sums are f32. With scores
 // of a standard deviation of two K's costs 3.5e-4 of the output's norm, the numerators' 2.0e-4, V's 1.6e-4 (an f16 output's own
-// is 2.1e-4). Exact K codes with their scales on the sums instead would take 12 multiplications for every 4 saved here with
-// three row blocks, a tenth of the kernel's time.
+// is 2.1e-4). Exact K codes with their scales on the sums, as yahkv_decode_attend has them, were built: the error of an f32
+// output falls from 4.9e-4 to 2.8e-4 (yahkv_decode_attend: 2.2e-4) and 64 sequences on 32K take 146 us instead of 122, 32 on 8K 44
+// instead of 39, 45 in 3 groups 31.5 instead of 28.5: four multiply-adds a row block for every four multiplications saved, on
+// sums that the matrix unit leaves in the other half of the register file.
 //
 // What bounds it: with few rows the reads and a workgroup's beginning and end (12 query rows on 32K keys of 4 x 256 dims: 23
 // us, 71 MB); with three row blocks of 256 dims the vector unit, which issues 1470 instructions of 4 cycles for a tile's 192
@@ -328,7 +332,8 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
     for (int dt = 0; dt < NDT; ++dt) o[i][dt] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   }
   for (int tile = tile0; tile < tile1; tile += step) {
-    // (the last tile's successor is itself: every pass issues the same loads, which keeps the waits exact)
+    // (the last tile's successor is itself: every pass issues the same loads, which keeps the waits exact where a tile has at
+    // most two pages)
 #pragma unroll
     for (int j = 0; j < PPT; ++j) pgc[j] = pgn[j];
     load_pages(tile + step < tile1 ? tile + step : tile, pgn);
