@@ -317,3 +317,28 @@ def test_a_group_led_by_sequences_shorter_than_its_prefix(yahkv, torch_gpu, lead
     check(torch, got, want, torch.float32)
     for s, m in enumerate(lens):
         assert m > 0 or not got[s].any()
+
+
+@pytest.mark.parametrize("fmt,n_q,n_kv,hd,pt", [(8, 24, 4, 256, 64), (8, 8, 2, 128, 16), (4, 32, 8, 128, 32), (4, 24, 4, 256, 64)])
+@pytest.mark.parametrize("bound", [0, 65536])
+@pytest.mark.parametrize("kind", ["keys", "keys next to ordinary ones", "scale", "no scale"])
+def test_scores_far_from_zero(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, bound, kind):
+    """Scores of 1e9 and 1e31, where a unit of their last place is far more than one (a softmax of them is its largest score's
+    key), and scores that are all next to nothing (a mean). Large keys are powers of two times their codes, so that they are
+    exact in f16 and the largest score is too."""
+    torch = torch_gpu
+    groups = [(192, [192, 250, 300, 0]), (0, [70, 1]), (640, [700] * 30)]
+    g, table, host, dev, lens, q, a = batch(yahkv, torch, fmt, n_q, n_kv, hd, pt, groups, hd + pt, fill=0x7F if kind == "keys" else 0x11)
+    scale = {"scale": 1e30, "no scale": 1e-38}.get(kind, hd ** -0.5)
+    if kind.startswith("keys"):
+        ks = dev.ks.view(torch.float16).view(-1, n_kv, pt, hd // 32)
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        some = torch.rand(ks.shape[:3], generator=gen, device="cuda") < (2.0 if kind == "keys" else 0.1)
+        ks.copy_(torch.where(some[..., None] & torch.isfinite(ks), torch.full_like(ks, 32768.0), ks))
+        for name, arr in host.arrays().items():
+            arr.reshape(-1)[:] = dev.numpy()[name].reshape(-1)
+        q *= 200.0
+    if bound:
+        a.update(max_shared_len=bound, max_tail_len=40000)
+    want = closed(g, table, host, lens, q.half().double().cpu().numpy(), scale)
+    check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=scale, **a), want, torch.float32)

@@ -44,11 +44,14 @@ namespace yahkv {
 namespace {
 
 constexpr int kSharedWaves = 4;
-constexpr float kNone = -1.0e30f;  // reference point of a row before its first tile
+constexpr float kNone = kNegMax;  // reference point of a row before its first tile
 // Numerators are 2^(score - m). m is a whole number, so that moving it rescales exactly, kBias below the largest score when
 // it was set, and is moved when a score exceeds it by kBias + kSlack: numerators stay within f16's range and those
 // 2^-24 of the largest are still normal numbers.
 constexpr float kBias = 10.0f, kSlack = 4.0f;
+// Scores beyond this (in powers of two) are rounded before m is subtracted, and m is the largest score itself: the distances
+// of a product that is not rounded from one that is, or of ten from a sum, come near one there and pass f16's range further out.
+constexpr float kFar = 0x1p20f;
 
 struct SharedArgs {
   Geom g;
@@ -199,15 +202,24 @@ struct QueryRows {
 
 // Numerators of one row block's tile: this lane's 16 keys 16 jg + 4 kt + r of its row, scores st in, second operand pv out.
 template <int D>
-__device__ __forceinline__ void Numerators(const f4v (&st)[4], float sscale, float& m, float& l, f4v (&o)[D / 16], h8v (&pv)[2]) {
+__device__ __forceinline__ void Numerators(f4v (&st)[4], float sscale, float& m, float& l, f4v (&o)[D / 16], h8v (&pv)[2]) {
   constexpr int NDT = D / 16;
   float mx = fmaxf(st[0][0], st[0][1]);
   mx = fmaxf(fmaxf(mx, st[0][2]), st[0][3]);
 #pragma unroll
   for (int kt = 1; kt < 4; ++kt) mx = fmaxf(fmaxf(mx, st[kt][0]), st[kt][1]), mx = fmaxf(fmaxf(mx, st[kt][2]), st[kt][3]);
   mx = OverLaneGroups(mx, [](float x, float y) { return fmaxf(x, y); }) * sscale;
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m + (kBias + kSlack)) != 0, 0)) {
-    const float mn = mx > m + (kBias + kSlack) ? __builtin_ceilf(mx) - kBias : m;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64((mx > m + (kBias + kSlack)) | (fabsf(mx) > kFar)) != 0, 0)) {
+    const bool far = __builtin_amdgcn_ballot_w64(fabsf(mx) > kFar) != 0;
+    if (far) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[kt][r] *= sscale;
+      sscale = 1.0f;
+    }
+    const float bias = far ? 0.0f : kBias, slack = far ? 0.0f : kBias + kSlack;
+    const float mn = mx > m + slack ? __builtin_ceilf(mx) - bias : m;
     const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn, l *= alpha;
     // (the rescaled accumulators go back through a matrix instruction with zero factors: that keeps them in the
@@ -398,7 +410,7 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (tile * kTile + 16 * jg + 4 * kt + r >= n_keys) st[i][kt][r] = kNegMax;
+            if (tile * kTile + 16 * jg + 4 * kt + r >= n_keys) st[i][kt][r] = -__builtin_inff();
       }
       Numerators<D>(st[i], tscale, m[i], l[i], o[i], pv[i]);
     }
