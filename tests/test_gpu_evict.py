@@ -100,6 +100,31 @@ def test_weights_of_a_large_batch(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt):
         assert m > 0 or not out[s].any()
 
 
+@pytest.mark.parametrize("fmt,n_q,n_kv,hd,pt,bound", [(8, 24, 4, 256, 64, 0), (8, 24, 4, 256, 64, 70001), (4, 32, 8, 128, 16, 0),
+                                                      (8, 8, 1, 256, 32, 70001), (4, 6, 3, 128, 64, 70001)])
+def test_weights_of_scores_far_from_zero(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, bound):
+    """Scores of 1e9, where a unit of their last place is 64: a row's largest has all of its weight (the others are millions
+    below it), and a key's weights are a whole number."""
+    torch = torch_gpu
+    lens = [700, 1, 0, 64, 65, 333, 2000, 17, 130]
+    g, table, host, dev, rng = setup(yahkv, torch, fmt, n_q, n_kv, hd, pt, lens, seed=hd + pt + n_kv, fill=0x7F)
+    n, T, scale = len(lens), max(lens), hd ** -0.5
+    ks = dev.ks.view(torch.float16)
+    ks.copy_(torch.where(torch.isfinite(ks), torch.full_like(ks, 32768.0), ks))
+    for name, arr in host.arrays().items():
+        arr.reshape(-1)[:] = dev.numpy()[name].reshape(-1)
+    q = torch.from_numpy(200 * rng.standard_normal((n, n_q, hd)).astype(np.float32)).cuda().half()
+    want, _ = exact_weights(g, table, host, lens, q.double().cpu().numpy(), scale)
+    assert np.all(np.abs(want - np.round(want)) < 1e-9)
+    w = torch.full((n, n_kv, (bound or T) + 2), -1.0, device="cuda")
+    out = yahkv.decode_attend_weights(dev, torch.from_numpy(table).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), bound or T, q,
+                                      scale, w)
+    check(torch, out, closed(g, table, host, lens, q.double().cpu().numpy(), scale), torch.float32)
+    for s, m in enumerate(lens):
+        assert np.array_equal(w[s, :, :m].double().cpu().numpy(), np.round(want[s, :, :m])), s
+        assert bool((w[s, :, m:] == -1.0).all())
+
+
 def test_weights_from_a_graph(yahkv, torch_gpu):
     torch = torch_gpu
     lens = [700, 64, 0, 333]

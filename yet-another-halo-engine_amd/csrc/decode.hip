@@ -114,7 +114,9 @@ void DattnPart(const DecodeArgs a) {
   constexpr bool Q8 = FMT == 8;
   constexpr int KW = Q8 ? 4 : 2;             // dwords of K codes per lane and block
   constexpr int NVB = Q8 ? NT / 2 : NB / 2;  // 16-byte V loads per lane and half of the dims
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  // kUnit: a row's maximum leaves in natural units. WEIGH's stays in powers of two, the scores' own: rounded on its way there and
+  // back it would be 64 off a score of 1e9, and every weight 2^64.
+  constexpr float kLog2e = 1.4426950408889634f, kUnit = WEIGH ? 1.0f : 0.6931471805599453f;
   const Geom g = a.g;
   const int G = g.group(), H = g.n_kv;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -409,7 +411,7 @@ void DattnPart(const DecodeArgs a) {
     for (int r = 0; r < 4; ++r) {
       const float l = HalfSum32(lsum[r]);
       const int head = 4 * half + r;
-      if (n32 == 0 && head < G) StoreDevice2(rml, head * 8, m[r] * kLn2, l);
+      if (n32 == 0 && head < G) StoreDevice2(rml, head * 8, m[r] * kUnit, l);
     }
     if (kg == 0 || kg == 2) {
 #pragma unroll
@@ -768,7 +770,7 @@ void DattnPart(const DecodeArgs a) {
           float l = 0.0f;
 #pragma unroll
           for (int w = 0; w < kWavesPerGroup; ++w) l += merge_l[w][gi];
-          StoreDevice2(rml, (d * G + gi) * 8, merge_m[gi] * kLn2, d == 0 ? l : 0.0f);
+          StoreDevice2(rml, (d * G + gi) * 8, merge_m[gi] * kUnit, d == 0 ? l : 0.0f);
         }
       }
       if (!FUSED) return;  // MODE 2: the separate merge dispatch takes it from here
@@ -800,7 +802,9 @@ __global__ __launch_bounds__(64 * kWavesPerGroup) __attribute__((amdgpu_waves_pe
 void DattnPartWhole(const DecodeArgs a) {
   constexpr int D = 256, PT = kTile, NB = D / 32, NT = D / 16, NVB = NT / 2, QE = NB * 32 / 64;
   constexpr int NTH = 64 * kWavesPerGroup;
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  // kUnit: a row's maximum leaves in natural units. WEIGH's stays in powers of two, the scores' own: rounded on its way there and
+  // back it would be 64 off a score of 1e9, and every weight 2^64.
+  constexpr float kLog2e = 1.4426950408889634f, kUnit = WEIGH ? 1.0f : 0.6931471805599453f;
   const Geom g = a.g;
   const int G = g.group(), H = g.n_kv;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -924,7 +928,7 @@ void DattnPartWhole(const DecodeArgs a) {
   auto flush = [&]() {
     const size_t part = PartialIndex(a, blockIdx.x, wave, cur) * G;
     const auto rml = DeviceBuffer(a.ml + part * 2), racc = DeviceBuffer(a.acc + part * D);
-    if (lane < G) StoreDevice2(rml, lane * 8, share_m[wave][lane] * kLn2, share_l[wave][lane]);
+    if (lane < G) StoreDevice2(rml, lane * 8, share_m[wave][lane] * kUnit, share_l[wave][lane]);
     for (int i = lane; i < G * D; i += 64) StoreDevice(racc, i * 4, share[i]);
     __builtin_amdgcn_wave_barrier();  // (the slot is rewritten for the next pair)
   };
@@ -1077,7 +1081,7 @@ void DattnPartWhole(const DecodeArgs a) {
       }
     }
     StoreDevice(racc, i * 4, v);
-    if (d < a.wpc) StoreDevice2(rml, (d * G + gi) * 8, M * kLn2, d == 0 ? l : 0.0f);
+    if (d < a.wpc) StoreDevice2(rml, (d * G + gi) * 8, M * kUnit, d == 0 ? l : 0.0f);
   }
 }
 
@@ -1149,7 +1153,7 @@ constexpr int kReduceThreads = 256;  // also the number of partial slots weighed
 constexpr int kReduceThreadsWide = 512;  // ... where a pair has more than that many places for partials
 constexpr int kReduceDepth = 4;      // partials a group loads together
 constexpr int kReduceMinDims = 32;   // fewest dims of a head one workgroup sums
-// WEIGH: yahkv_decode_attend_weights' form: out of any type, and every row's maximum and sum.
+// WEIGH: yahkv_decode_attend_weights' form: out of any type, maxima in powers of two, and every row's maximum and sum left.
 template <int RT, bool WEIGH>
 __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const StepRows rows) {
   const Geom g = a.g;
@@ -1230,7 +1234,7 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
       n += wave_n[w];
     }
     if (l > 0.0f) {
-      const float w = __expf(m - M);
+      const float w = WEIGH ? __builtin_amdgcn_exp2f(m - M) : __expf(m - M);
       wgt[at] = w, wl[at] = w * l, slot[at] = t;
     }
     __syncthreads();
@@ -1272,7 +1276,7 @@ __global__ __launch_bounds__(RT) void DattnReduce(const DecodeArgs a, const Step
 
 // ---- the weights --------------------------------------------------------------------------------------------------------
 
-// weights_out[s][h][t] = decay * weights_in[s][h][t] + sum over the head's query rows of e^(score - M) / l: a thread per
+// weights_out[s][h][t] = decay * weights_in[s][h][t] + sum over the head's query rows of 2^(score - M) / l: a thread per
 // key, the rows' maxima and sums the same for a workgroup. Reads 4 G + 4 and writes 4 bytes a key, a tenth of what the
 // key's K and V rows take (24 ragged sequences of up to 16K, 32 + 8 heads of 128 dims in 4 bits: 9.4 us beside the part
 // kernel's 70, of which leaving the scores takes 3).
@@ -1291,7 +1295,6 @@ __global__ __launch_bounds__(kWeighThreads) void WeighKeys(const WeighArgs a) {
   const int len = min(max(a.seq_len[s], 0), a.max_len);
   const int t = blockIdx.x * kWeighThreads + threadIdx.x;
   if (t >= len) return;
-  constexpr float kLog2e = 1.4426950408889634f;
   const size_t q0 = size_t(s) * a.n_q + size_t(h) * G;
   float sc[kMaxGroup];
 #pragma unroll
@@ -1303,7 +1306,7 @@ __global__ __launch_bounds__(kWeighThreads) void WeighKeys(const WeighArgs a) {
   for (int r = 0; r < kMaxGroup; ++r) {
     if (r >= G) break;
     const float* ml = a.row_ml + (q0 + r) * 2;
-    p += __builtin_amdgcn_exp2f(__builtin_fmaf(-kLog2e, ml[0], sc[r])) / ml[1];
+    p += __builtin_amdgcn_exp2f(sc[r] - ml[0]) / ml[1];
   }
   a.out[at] = w + p;
 }

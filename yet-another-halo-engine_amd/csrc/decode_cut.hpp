@@ -61,7 +61,7 @@ struct DecodeArgs {
   int32_t tile_mult;
   int32_t out_dtype;  // of out (yahkv_dtype): F32 for every entry point that has no argument for it
   // yahkv_decode_attend_weights: the part kernel leaves every key's score (in base-2 units, scale applied), f32
-  // [n_seqs][n_q][score_stride], and the merge every query row's maximum (natural units) and sum, f32 [n_seqs][n_q][2]
+  // [n_seqs][n_q][score_stride], and the merge every query row's maximum (in the same units) and sum, f32 [n_seqs][n_q][2]
   float* scores;
   float* row_ml;
   int32_t score_stride;
