@@ -49,8 +49,9 @@ constexpr float kNone = kNegMax;  // reference point of a row before its first t
 // it was set, and is moved when a score exceeds it by kBias + kSlack: numerators stay within f16's range and those
 // 2^-24 of the largest are still normal numbers.
 constexpr float kBias = 10.0f, kSlack = 4.0f;
-// Scores beyond this (in powers of two) are rounded before m is subtracted, and m is the largest score itself: the distances
-// of a product that is not rounded from one that is, or of ten from a sum, come near one there and pass f16's range further out.
+// Scores are rounded before m is subtracted (an unrounded product, as in a multiply-add, is half a unit of the last place off
+// the largest score: 32 at 2^30, far past f16's range), and where they are beyond kFar m is the largest score itself (from 2^27
+// on ten below it need not be a float).
 constexpr float kFar = 0x1p20f;
 
 struct SharedArgs {
@@ -202,24 +203,16 @@ struct QueryRows {
 
 // Numerators of one row block's tile: this lane's 16 keys 16 jg + 4 kt + r of its row, scores st in, second operand pv out.
 template <int D>
-__device__ __forceinline__ void Numerators(f4v (&st)[4], float sscale, float& m, float& l, f4v (&o)[D / 16], h8v (&pv)[2]) {
+__device__ __forceinline__ void Numerators(const f4v (&st)[4], float sscale, float& m, float& l, f4v (&o)[D / 16], h8v (&pv)[2]) {
+#pragma clang fp contract(off)
   constexpr int NDT = D / 16;
   float mx = fmaxf(st[0][0], st[0][1]);
   mx = fmaxf(fmaxf(mx, st[0][2]), st[0][3]);
 #pragma unroll
   for (int kt = 1; kt < 4; ++kt) mx = fmaxf(fmaxf(mx, st[kt][0]), st[kt][1]), mx = fmaxf(fmaxf(mx, st[kt][2]), st[kt][3]);
   mx = OverLaneGroups(mx, [](float x, float y) { return fmaxf(x, y); }) * sscale;
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64((mx > m + (kBias + kSlack)) | (fabsf(mx) > kFar)) != 0, 0)) {
-    const bool far = __builtin_amdgcn_ballot_w64(fabsf(mx) > kFar) != 0;
-    if (far) {
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[kt][r] *= sscale;
-      sscale = 1.0f;
-    }
-    const float bias = far ? 0.0f : kBias, slack = far ? 0.0f : kBias + kSlack;
-    const float mn = mx > m + slack ? __builtin_ceilf(mx) - bias : m;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx - m > kBias + kSlack) != 0, 0)) {
+    const float mn = mx - m > kBias + kSlack ? __builtin_ceilf(mx) - (fabsf(mx) > kFar ? 0.0f : kBias) : m;
     const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn, l *= alpha;
     // (the rescaled accumulators go back through a matrix instruction with zero factors: that keeps them in the
@@ -240,7 +233,7 @@ __device__ __forceinline__ void Numerators(f4v (&st)[4], float sscale, float& m,
   for (int kt = 0; kt < 4; ++kt) {
     float p[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][r], sscale, -m));
+    for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(st[kt][r] * sscale - m);
     const h2v p0 = {static_cast<_Float16>(p[0]), static_cast<_Float16>(p[1])};
     const h2v p1 = {static_cast<_Float16>(p[2]), static_cast<_Float16>(p[3])};
     // (the sum is of the rounded numerators, as the second product's is)
