@@ -29,8 +29,8 @@
 // sums that the matrix unit leaves in the other half of the register file.
 //
 // What bounds it: with few rows the reads and a workgroup's beginning and end (12 query rows on 32K keys of 4 x 256 dims: 23
-// us, 71 MB); with three row blocks of 256 dims the vector unit, which issues 1470 instructions of 4 cycles for a tile's 192
-// matrix instructions of 16 and is busy with 900 of them decoding (384 rows x 32K keys: 97 us, 0.53 PFLOP/s, 4.5 us a tile of
+// us, 71 MB); with three row blocks of 256 dims the vector unit, which issues 1520 instructions of 4 cycles for a tile's 192
+// matrix instructions of 16 and is busy with 900 of them decoding (384 rows x 32K keys: 98 us, 0.53 PFLOP/s, 4.5 us a tile of
 // each wave, of which a matrix product at this card's rate would take 2.7). Three row blocks are what fits: accumulators 192
 // registers, queries 96, codes 64, scores 48. Decoding once for four waves of other rows, through LDS, brings a tile to 3.2 us, but
 // then no two waves share rows, and writing four times the partials and reading them again takes all of it back.
