@@ -342,3 +342,18 @@ def test_scores_far_from_zero(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt, bound, k
         a.update(max_shared_len=bound, max_tail_len=40000)
     want = closed(g, table, host, lens, q.half().double().cpu().numpy(), scale)
     check(torch, yahkv.decode_attend_shared(dev, q=q.half(), scale=scale, **a), want, torch.float32)
+
+
+@pytest.mark.parametrize("fmt,n_q,n_kv,hd,pt", [(8, 24, 4, 256, 64), (8, 8, 2, 128, 16), (4, 32, 8, 128, 32), (4, 24, 4, 256, 64)])
+def test_unwritten_slots_have_no_say(yahkv, torch_gpu, fmt, n_q, n_kv, hd, pt):
+    """The same bits whatever the slots behind every sequence's end hold: zeros, ordinary codes and scales, NaN, large scales. (The
+    written keys are small ones, whose scales do not survive a factor of 2^-7 in f16.)"""
+    torch = torch_gpu
+    got = []
+    for fill in (0x00, 0x21, 0x7F, 0xFF, 0x7B):
+        g, table, host, dev, lens, q, a = batch(yahkv, torch, fmt, n_q, n_kv, hd, pt, [(192, [192, 250, 300, 0]), (0, [70, 1]), (640, [700, 641])],
+                                                hd, fill=fill)
+        dev.ks.view(torch.float16).mul_(0.01)
+        got.append(yahkv.decode_attend_shared(dev, q=(q * 100).half(), scale=hd ** -0.5, **a))
+    for x in got[1:]:
+        assert torch.equal(x, got[0])

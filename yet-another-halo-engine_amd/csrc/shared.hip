@@ -142,8 +142,8 @@ __device__ __forceinline__ void SetSaturation(bool on) {
 // K's do not: a saturated product would be another score, and an infinite one a NaN. A tile with a large scale enters the
 // product with all its scales times 2^-7, and its scores are multiplied by 2^7 behind it. That is exact but for scales below
 // 2^-7, those of ordinary keys in such a tile, which become whole multiples of 2^-24: 2^-18 off at most, which is to keys of
-// values about one what f16's rounding of them is. k: the tile's scales, eight a lane (those of keys behind the end may be
-// anything: what they hold costs this path and changes nothing). Returns whether it is such a tile.
+// values about one what f16's rounding of them is. k: the tile's scales, eight a lane (0 for keys behind the end, so that what
+// they hold has no say in it). Returns whether it is such a tile.
 __device__ __forceinline__ bool ShrinkLargeKeys(uint4& k) {
   const uint32_t most = Larger(__builtin_elementwise_max(Magnitudes(k.x, k.y), Magnitudes(k.z, k.w)));
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kLargeScale) == 0, 1)) return false;
@@ -345,13 +345,16 @@ __device__ __forceinline__ void StreamKeys(const SharedArgs& a, const int32_t* r
     const bool cut = (tile + 1) * kTile > n_keys;
     bool saturates;
     int up = 0;  // this tile's scores come times 2^-up
-    {  // scales to LDS; the V scales of masked keys become 0, which makes their V rows 0 whatever they hold
+    {  // scales to LDS; those of masked keys become 0, which makes their V rows 0 whatever they hold
       uint32_t w[4] = {vsr.x, vsr.y, vsr.z, vsr.w};
       if (cut) {
         const int k0 = tile * kTile + 8 * (lane % 8);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (k0 + e >= n_keys) w[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        const int key = tile * kTile + lane * 8 / NB;  // K's: a lane has all of a key, or of two
+        if (key >= n_keys) ksr.x = ksr.y = 0u;
+        if (key + (NB == 4 ? 1 : 0) >= n_keys) ksr.z = ksr.w = 0u;
       }
       if (ShrinkLargeKeys(ksr)) up = 7;
       if (lane < NB * 8) {
